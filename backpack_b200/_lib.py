@@ -88,6 +88,10 @@ SIGNATURES["bpq4k_kq_matmul_moe_f32"] = (C.c_int, [vp, C.c_int, vp, vp, vp, vp, 
 SIGNATURES["bpq4k_moe_ffn_work_floats"] = (C.c_uint64, [u32, u32, u32, u32])
 SIGNATURES["bpq4k_moe_ffn_f32"] = (C.c_int, [vp, C.c_int, vp, vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, u32, vp, C.c_uint64, vp])
 SIGNATURES["bpq4k_kq_respace_device"] = (C.c_int, [vp, C.c_int, vp, u32, u32, vp, vp])
+SIGNATURES["bpq4k_add_rmsnorm_i8"] = (C.c_int, [vp, C.c_int, vp, vp, vp, C.c_float, vp, vp, vp, u32, u32, u32, u32, u32, u32, vp])
+SIGNATURES["bpq4k_quantize_i8"] = (C.c_int, [vp, C.c_int, vp, vp, vp, u32, u32, u32, u32, vp])
+SIGNATURES["bpq4k_matmul_i8"] = (C.c_int, [vp, C.c_int, vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, u32, u32, vp])
+SIGNATURES["bpq4k_logprobs"] = (C.c_int, [vp, C.c_int, vp, u32, u32, u32, vp, u32, vp, vp, u32, vp, vp, vp])
 
 _lib = None
 

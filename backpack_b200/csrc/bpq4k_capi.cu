@@ -1015,6 +1015,134 @@ int bpq4k_argmax_f32(bpq4k_handle_t h, const float* logits, uint32_t n, int32_t*
     return BPQ4K_OK;
 }
 
+// ---- the 8-bit path ----------------------------------------------------------
+
+namespace {
+
+// Bytes of an element, 0 for a type these operators do not take.
+uint32_t ftype_bytes(int ftype) { return ftype == BPQ4K_TYPE_F32 ? 4u : ftype == BPQ4K_TYPE_F16 || ftype == BPQ4K_TYPE_BF16 ? 2u : 0u; }
+bool aligned_to(const void* p, uint32_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// Rows of `n` elements, ld apart; what every operator of the path asks of them.
+int check_rows(bpq4k_context* h, const char* name, const void* p, uint32_t n, uint32_t ld, uint32_t align) {
+    if (!p) return fail(h, BPQ4K_ERR_INVALID_ARG, "%s is null", name);
+    if (ld < n) return fail(h, BPQ4K_ERR_INVALID_ARG, "the rows of %s are %u apart, shorter than their %u values", name, ld, n);
+    if (!aligned_to(p, align)) return fail(h, BPQ4K_ERR_MISALIGNED, "%s is not %u-byte aligned", name, align);
+    return BPQ4K_OK;
+}
+int check_codes(bpq4k_context* h, const char* name, const void* p, uint32_t K, uint32_t ld) {
+    if (int s = check_rows(h, name, p, K, ld, 16u)) return s;
+    if (ld % 16u) return fail(h, BPQ4K_ERR_MISALIGNED, "the rows of %s are %u bytes apart, not a multiple of 16", name, ld);
+    return BPQ4K_OK;
+}
+int check_floats(bpq4k_context* h, const char* name, const void* p) {
+    if (!p) return fail(h, BPQ4K_ERR_INVALID_ARG, "%s is null", name);
+    if (!aligned_to(p, 4u)) return fail(h, BPQ4K_ERR_MISALIGNED, "%s is not 4-byte aligned", name);
+    return BPQ4K_OK;
+}
+
+int rows_i8(bpq4k_context* h, int ftype, const RowsI8Args& a, cudaStream_t st) {
+    const uint32_t es = ftype_bytes(ftype);
+    if (!es) return fail(h, BPQ4K_ERR_UNSUPPORTED, "element type %d is not F32 (0), F16 (1) or BF16 (30)", ftype);
+    if (a.M == 0) return BPQ4K_OK;
+    if (a.K == 0 || a.K > kRowsI8MaxK) return fail(h, BPQ4K_ERR_UNSUPPORTED, "K=%u is not between 1 and %u", a.K, kRowsI8MaxK);
+    if (a.M > 0x7FFFFFFFu) return fail(h, BPQ4K_ERR_UNSUPPORTED, "M=%u is more than 2^31 - 1 rows", a.M);
+    if (int s = check_rows(h, "X", a.X, a.K, a.ldx, es)) return s;
+    if (a.R)
+        if (int s = check_rows(h, "residual", a.R, a.K, a.ldr, es)) return s;
+    if (a.sum)
+        if (int s = check_rows(h, "sum", a.sum, a.K, a.lds, es)) return s;
+    if (int s = check_codes(h, "codes", a.codes, a.K, a.ldc)) return s;
+    if (int s = check_floats(h, "scales", a.scales)) return s;
+    DeviceGuard g(h->device);
+    const cudaError_t e = launch_rows_i8(a, ftype, st);
+    h->launches += 1;
+    if (e != cudaSuccess) return cuda_fail(h, e, "8-bit rows launch");
+    return BPQ4K_OK;
+}
+
+}  // namespace
+
+int bpq4k_add_rmsnorm_i8(bpq4k_handle_t h, int ftype, const void* X, const void* residual, const float* weight, float eps,
+                         void* sum, int8_t* codes, float* scales, uint32_t M, uint32_t K, uint32_t ldx, uint32_t ldr,
+                         uint32_t lds, uint32_t ldc, void* stream) {
+    if (!h) return BPQ4K_ERR_INVALID_ARG;
+    if (M)
+        if (int s = check_floats(h, "weight", weight)) return s;
+    if (sum && !residual) return fail(h, BPQ4K_ERR_INVALID_ARG, "sum without a residual");
+    if (!(eps >= 0.f)) return fail(h, BPQ4K_ERR_INVALID_ARG, "eps is negative or not a number");
+    RowsI8Args a{};
+    a.X = X, a.R = residual, a.w = weight, a.sum = sum, a.codes = codes, a.scales = scales;
+    a.M = M, a.K = K, a.ldx = ldx, a.ldr = ldr, a.lds = lds, a.ldc = ldc, a.eps = eps, a.status = h->dev_status;
+    return rows_i8(h, ftype, a, static_cast<cudaStream_t>(stream));
+}
+
+int bpq4k_quantize_i8(bpq4k_handle_t h, int ftype, const void* X, int8_t* codes, float* scales, uint32_t M, uint32_t K,
+                      uint32_t ldx, uint32_t ldc, void* stream) {
+    if (!h) return BPQ4K_ERR_INVALID_ARG;
+    RowsI8Args a{};
+    a.X = X, a.codes = codes, a.scales = scales, a.M = M, a.K = K, a.ldx = ldx, a.ldc = ldc, a.status = h->dev_status;
+    return rows_i8(h, ftype, a, static_cast<cudaStream_t>(stream));
+}
+
+int bpq4k_matmul_i8(bpq4k_handle_t h, int ftype, const int8_t* X, const float* x_scales, const int8_t* W, const float* w_scales,
+                    const float* bias, void* Y, uint32_t M, uint32_t N, uint32_t K, uint32_t ldx, uint32_t ldw, uint32_t ldy,
+                    void* stream) {
+    if (!h) return BPQ4K_ERR_INVALID_ARG;
+    const uint32_t es = ftype_bytes(ftype);
+    if (!es) return fail(h, BPQ4K_ERR_UNSUPPORTED, "element type %d is not F32 (0), F16 (1) or BF16 (30)", ftype);
+    if (M == 0 || N == 0) return BPQ4K_OK;
+    if (K == 0 || K > kMatmulI8MaxK) return fail(h, BPQ4K_ERR_UNSUPPORTED, "K=%u is not between 1 and %u", K, kMatmulI8MaxK);
+    if (M > kMatmulI8MaxRows || N > kMatmulI8MaxRows)
+        return fail(h, BPQ4K_ERR_UNSUPPORTED, "M=%u or N=%u is more than %u", M, N, kMatmulI8MaxRows);
+    if (int s = check_codes(h, "X", X, K, ldx)) return s;
+    if (int s = check_codes(h, "W", W, K, ldw)) return s;
+    if (int s = check_rows(h, "Y", Y, N, ldy, es)) return s;
+    if (int s = check_floats(h, "x_scales", x_scales)) return s;
+    if (int s = check_floats(h, "w_scales", w_scales)) return s;
+    if (bias)
+        if (int s = check_floats(h, "bias", bias)) return s;
+    DeviceGuard g(h->device);
+    MatmulI8Args a{};
+    a.X = X, a.xs = x_scales, a.W = W, a.ws = w_scales, a.bias = bias, a.Y = Y;
+    a.M = M, a.N = N, a.K = K, a.ldx = ldx, a.ldw = ldw, a.ldy = ldy;
+    int launches = 0;
+    const cudaError_t e = launch_matmul_i8(a, ftype, h->dev_status, h->sm_count, static_cast<cudaStream_t>(stream), &launches);
+    h->launches += (uint64_t)launches;
+    if (e != cudaSuccess) return cuda_fail(h, e, "8-bit matmul launch");
+    return BPQ4K_OK;
+}
+
+int bpq4k_logprobs(bpq4k_handle_t h, int ftype, const void* logits, uint32_t M, uint32_t V, uint32_t ld, const int32_t* given,
+                   uint32_t nGiven, float* given_lp, float* entropy, uint32_t nTop, int32_t* top_ids, float* top_lp, void* stream) {
+    if (!h) return BPQ4K_ERR_INVALID_ARG;
+    const uint32_t es = ftype_bytes(ftype);
+    if (!es) return fail(h, BPQ4K_ERR_UNSUPPORTED, "element type %d is not F32 (0), F16 (1) or BF16 (30)", ftype);
+    if (M == 0) return BPQ4K_OK;
+    if (V == 0 || V > 0x7FFFFFFFu || M > 0x7FFFFFFFu) return fail(h, BPQ4K_ERR_UNSUPPORTED, "M=%u or V=%u is not between 1 and 2^31 - 1", M, V);
+    if (nTop > kLogprobsMaxTop || nTop > V) return fail(h, BPQ4K_ERR_UNSUPPORTED, "nTop=%u is more than %u or than V=%u", nTop, kLogprobsMaxTop, V);
+    if (int s = check_rows(h, "logits", logits, V, ld, es)) return s;
+    if (nGiven) {
+        if (int s = check_floats(h, "given", given)) return s;
+        if (int s = check_floats(h, "given_lp", given_lp)) return s;
+    }
+    if (entropy)
+        if (int s = check_floats(h, "entropy", entropy)) return s;
+    if (nTop) {
+        if (int s = check_floats(h, "top_ids", top_ids)) return s;
+        if (int s = check_floats(h, "top_lp", top_lp)) return s;
+    }
+    if (!nGiven && !entropy && !nTop) return fail(h, BPQ4K_ERR_INVALID_ARG, "nothing is asked of the logits");
+    DeviceGuard g(h->device);
+    LogprobsArgs a{};
+    a.logits = logits, a.given = given, a.given_lp = given_lp, a.entropy = entropy, a.top_ids = top_ids, a.top_lp = top_lp;
+    a.M = M, a.V = V, a.ld = ld, a.nGiven = nGiven, a.nTop = nTop;
+    const cudaError_t e = launch_logprobs(a, ftype, static_cast<cudaStream_t>(stream));
+    h->launches += 1;
+    if (e != cudaSuccess) return cuda_fail(h, e, "log probability launch");
+    return BPQ4K_OK;
+}
+
 int bpq4k_matmul_moe_f32(bpq4k_handle_t h, const float* X, const void* W, const float* bias, float* Y,
                          const uint32_t* offsets, const uint32_t* x_rows, uint32_t nSlots, uint32_t N, uint32_t K,
                          uint32_t rowStrideWords, uint32_t wRows, void* stream) {

@@ -161,6 +161,51 @@ double prefill_estimate_us(uint32_t M, uint32_t N, uint32_t K, int sm_count, int
 cudaError_t launch_rows_tc(const MatmulArgs& a, void* buffer, size_t buffer_bytes, int* status_dev,
                            int sm_count, TmapCache* tmaps, bool pdl, cudaStream_t stream, int* launches, int qtype = 12);
 
+// Rows to 8 bits (i8_rows.cu): v = X + R, p = v * w, codes = round(127 p / max|p|), scales = max|p| / sqrt(mean(v^2) + eps) / 127.
+// w null: p = v and no norm (R null then too).  sum (may be null): v, rounded to the element type; may be X or R themselves.
+// Element types are GGUF numbers: 0 float, 1 half, 30 bfloat16.  codes 16-byte aligned, ldc a multiple of 16.
+constexpr uint32_t kRowsI8MaxK = 32768;
+struct RowsI8Args {
+    const void* X;
+    const void* R;      // may be null
+    const float* w;     // may be null
+    void* sum;          // may be null
+    int8_t* codes;
+    float* scales;
+    uint32_t M, K, ldx, ldr, lds, ldc;
+    float eps;
+    int* status;        // debug build
+};
+cudaError_t launch_rows_i8(const RowsI8Args& a, int ftype, cudaStream_t stream);
+
+// Y[m*ldy + n] = (sum_k X[m*ldx + k] * W[n*ldw + k]) * xs[m] * ws[n] + bias[n], the sum exact in 32 bits (i8_matmul.cu).
+// X and W 16-byte aligned, ldx and ldw multiples of 16.
+constexpr uint32_t kMatmulI8MaxK = 131071;  // 128 * 128 * K stays below 2^31
+constexpr uint32_t kMatmulI8MaxRows = 1u << 24;
+struct MatmulI8Args {
+    const int8_t* X;
+    const float* xs;
+    const int8_t* W;
+    const float* ws;
+    const float* bias;  // may be null
+    void* Y;
+    uint32_t M, N, K, ldx, ldw, ldy;
+};
+cudaError_t launch_matmul_i8(const MatmulI8Args& a, int ftype, int* status_dev, int sm_count, cudaStream_t stream, int* launches);
+
+// Log probabilities of given tokens, entropy, most likely tokens of every row of logits (bpq4k_logprobs.cu).
+constexpr uint32_t kLogprobsMaxTop = 32;
+struct LogprobsArgs {
+    const void* logits;
+    const int32_t* given;  // [M][nGiven]
+    float* given_lp;       // [M][nGiven]
+    float* entropy;        // [M], may be null
+    int32_t* top_ids;      // [M][nTop]
+    float* top_lp;         // [M][nTop]
+    uint32_t M, V, ld, nGiven, nTop;
+};
+cudaError_t launch_logprobs(const LogprobsArgs& a, int ftype, cudaStream_t stream);
+
 // Cross-GPU barrier on flag words in peer memory (one process per GPU): store `epoch` into slot
 // `rank` of every peer's flag array, then wait -- at most timeout_cycles -- until every slot of the
 // own array has reached `epoch`.  On a time-out the kernel stores kDeviceTimeout to *status.

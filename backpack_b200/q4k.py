@@ -28,6 +28,10 @@ Q4_K, Q5_K, Q6_K = 12, 13, 14
 # Q6_K with every block padded to 224 bytes: the layout of the fast single-row Q6_K kernel (no reference counterpart)
 Q6_K_PADDED = 0x10E
 
+# element types of the 8-bit path's activations and of logits
+F32, F16, BF16 = 0, 1, 30
+LOGPROBS_MAX_TOP = 32
+
 OPT_GEMV_VARIANT = 1
 OPT_PREFILL_MODE = 2
 OPT_PREFILL_MIN_M = 3
@@ -139,6 +143,31 @@ class Q4KWeight:
         return Q4KWeight(self.buf[n0 * rb:n1 * rb], n1 - n0, self.K, self.rowStrideWords, self.qtype)
 
 
+@dataclass
+class I8Rows:
+    """Rows of 8-bit codes with one scale per row: a token's activations, or a weight matrix (a row per output channel).
+    Row m stands for codes[m] * scales[m]."""
+    codes: "torch.Tensor"     # int8 [rows, K]; rows begin at multiples of 16 bytes (stride(0) a multiple of 16)
+    scales: "torch.Tensor"    # float32 [rows]
+
+    @property
+    def K(self) -> int:
+        return self.codes.shape[1]
+
+    def rows(self, n0: int, n1: int) -> "I8Rows":
+        """A contiguous row range [n0, n1) as a view."""
+        return I8Rows(self.codes[n0:n1], self.scales[n0:n1])
+
+
+@dataclass
+class LogProbs:
+    """What ``Q4KContext.logprobs`` returns; fields that were not asked for are None."""
+    given: "torch.Tensor"     # float32, shape of `given`
+    entropy: "torch.Tensor"   # float32 [M]
+    top_ids: "torch.Tensor"   # int32 [M, top]
+    top: "torch.Tensor"       # float32 [M, top]
+
+
 class Q4KContext:
     """One handle on one device; not thread-safe (like the reference's GPUContext)."""
 
@@ -155,6 +184,7 @@ class Q4KContext:
         if st:
             raise Q4KError(st, "bpq4k_create")
         self.h = h
+        self._ftype = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
     def close(self) -> None:
         if getattr(self, "h", None):
@@ -288,6 +318,133 @@ class Q4KContext:
             out = torch.empty(1, dtype=torch.int32, device=logits.device)
         self._check(self.lib.bpq4k_argmax_f32(self.h, logits.data_ptr(), logits.numel(), out.data_ptr(), self._stream()))
         return out
+
+    # -- the 8-bit path ----------------------------------------------------
+    def _rows(self, t, name: str, dtype=None):
+        """(tensor as rows, element type number or 0, distance between rows) of an operand whose last dimension is contiguous."""
+        if not t.is_cuda or t.device.index != self.device:
+            raise ValueError(f"{name} is not on cuda:{self.device}")
+        if t.dim() != 2:
+            t = t.view(-1, t.shape[-1])
+        if dtype is None:
+            if t.dtype not in self._ftype:
+                raise ValueError(f"{name} is {t.dtype}, not float32, float16 or bfloat16")
+        elif t.dtype != dtype:
+            raise ValueError(f"{name} is {t.dtype}, not {dtype}")
+        m, k = t.shape
+        if k > 1 and t.stride(1) != 1:
+            raise ValueError(f"the values of a row of {name} are not contiguous")
+        ld = t.stride(0) if m > 1 else max(t.stride(0), k)
+        if ld >= 1 << 32 or m >= 1 << 32:
+            raise ValueError(f"{name} has more rows, or rows further apart, than 32 bits hold")
+        return t, self._ftype.get(t.dtype, 0), ld
+
+    def _floats(self, t, name: str, n: int):
+        """Address of n contiguous floats (None: none)."""
+        if t is None:
+            return None
+        if t.dtype != self._torch.float32 or t.device.index != self.device or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{name} is not {n} contiguous float32 values on cuda:{self.device}")
+        return t.data_ptr()
+
+    def _i8_out(self, m: int, k: int, out):
+        """The codes and scales a call writes: rows 16 bytes apart, or the caller's."""
+        torch = self._torch
+        if out is None:
+            dev = f"cuda:{self.device}"
+            return I8Rows(torch.empty((m, (k + 15) // 16 * 16), dtype=torch.int8, device=dev)[:, :k],
+                          torch.empty(m, dtype=torch.float32, device=dev))
+        if tuple(out.codes.shape) != (m, k):
+            raise ValueError(f"out holds rows {tuple(out.codes.shape)}, the call makes {(m, k)}")
+        return out
+
+    def add_rmsnorm_i8(self, x, weight, eps: float, residual=None, sum_out=None, out=None):
+        """Residual addition, RMSNorm and quantisation of the rows of x [..., K] to 8 bits (bpq4k_add_rmsnorm_i8).
+        Returns (I8Rows, x + residual); the sum is x itself without a residual.  `sum_out` may be x or residual."""
+        torch = self._torch
+        x, ft, ldx = self._rows(x, "x")
+        m, k = x.shape
+        pr = ps = None
+        ldr = lds = 0
+        total = x
+        if residual is not None:
+            residual, _, ldr = self._rows(residual, "residual", x.dtype)
+            total = torch.empty((m, k), dtype=x.dtype, device=x.device) if sum_out is None else sum_out
+            ts, _, lds = self._rows(total, "sum_out", x.dtype)
+            if residual.shape != x.shape or ts.shape != x.shape:
+                raise ValueError("x, residual and sum_out differ in shape")
+            pr, ps = residual.data_ptr(), ts.data_ptr()
+        elif sum_out is not None:
+            raise ValueError("sum_out without a residual")
+        out = self._i8_out(m, k, out)
+        codes, _, ldc = self._rows(out.codes, "codes", torch.int8)
+        self._check(self.lib.bpq4k_add_rmsnorm_i8(
+            self.h, ft, x.data_ptr(), pr, self._floats(weight, "weight", k), float(eps), ps, codes.data_ptr(),
+            self._floats(out.scales, "scales", m), m, k, ldx, ldr, lds, ldc, self._stream()))
+        return out, total
+
+    def quantize_i8(self, x, out=None) -> I8Rows:
+        """The rows of x [..., K] in 8 bits, a scale per row (bpq4k_quantize_i8)."""
+        x, ft, ldx = self._rows(x, "x")
+        m, k = x.shape
+        out = self._i8_out(m, k, out)
+        codes, _, ldc = self._rows(out.codes, "codes", self._torch.int8)
+        self._check(self.lib.bpq4k_quantize_i8(self.h, ft, x.data_ptr(), codes.data_ptr(), self._floats(out.scales, "scales", m),
+                                               m, k, ldx, ldc, self._stream()))
+        return out
+
+    def i8_weight(self, w: Q4KWeight) -> I8Rows:
+        """A K-quant weight in 8 bits, a scale per output channel: dequantised some rows at a time and quantised again."""
+        torch = self._torch
+        out = self._i8_out(w.N, w.K, None)
+        step = max(1, (16 << 20) // w.K)
+        part = torch.empty((min(step, w.N), w.K), dtype=torch.float32, device=w.buf.device)
+        for n in range(0, w.N, step):
+            end = min(n + step, w.N)
+            self.quantize_i8(self.dequant(w.rows(n, end), part[:end - n]), out.rows(n, end))
+        return out
+
+    def matmul_i8(self, x: I8Rows, w: I8Rows, bias=None, out=None, dtype=None):
+        """Y[m,n] = sum_k x[m,k] * w[n,k] + bias[n] of two matrices in 8 bits; Y float32, or `dtype`, or `out` (bpq4k_matmul_i8)."""
+        torch = self._torch
+        xc, _, ldx = self._rows(x.codes, "x", torch.int8)
+        wc, _, ldw = self._rows(w.codes, "w", torch.int8)
+        (m, k), n = xc.shape, wc.shape[0]
+        if wc.shape[1] != k:
+            raise ValueError(f"x has K={k}, the weight has K={wc.shape[1]}")
+        if out is None:
+            out = torch.empty((m, n), dtype=dtype or torch.float32, device=xc.device)
+        elif dtype is not None and out.dtype != dtype:
+            raise ValueError(f"out is {out.dtype}, not {dtype}")
+        y, ft, ldy = self._rows(out, "out")
+        if y.shape != (m, n):
+            raise ValueError(f"out holds {tuple(y.shape)}, the product is {(m, n)}")
+        self._check(self.lib.bpq4k_matmul_i8(
+            self.h, ft, xc.data_ptr(), self._floats(x.scales, "x.scales", m), wc.data_ptr(), self._floats(w.scales, "w.scales", n),
+            self._floats(bias, "bias", n), y.data_ptr(), m, n, k, ldx, ldw, ldy, self._stream()))
+        return out
+
+    def logprobs(self, logits, given=None, top: int = 0) -> LogProbs:
+        """Log probabilities of given tokens ([M] or [M, G] int32), entropy and the `top` most likely tokens of each row of logits
+        [M, V] (bpq4k_logprobs)."""
+        torch = self._torch
+        x, ft, ld = self._rows(logits, "logits")
+        m, v = x.shape
+        g, lp = 0, None
+        if given is not None:
+            if given.dtype != torch.int32 or given.device.index != self.device or not given.is_contiguous() or given.dim() not in (1, 2) or given.shape[0] != m:
+                raise ValueError(f"given is not contiguous int32 [{m}] or [{m}, tokens] on cuda:{self.device}")
+            g = given.shape[1] if given.dim() == 2 else 1
+            lp = torch.empty(given.shape, dtype=torch.float32, device=x.device)
+        if not 0 <= top <= LOGPROBS_MAX_TOP:
+            raise ValueError(f"top={top} is not between 0 and {LOGPROBS_MAX_TOP}")
+        entropy = torch.empty(m, dtype=torch.float32, device=x.device)
+        ids = torch.empty((m, top), dtype=torch.int32, device=x.device) if top else None
+        best = torch.empty((m, top), dtype=torch.float32, device=x.device) if top else None
+        self._check(self.lib.bpq4k_logprobs(
+            self.h, ft, x.data_ptr(), m, v, ld, given.data_ptr() if g else None, g, lp.data_ptr() if g else None, entropy.data_ptr(),
+            top, ids.data_ptr() if top else None, best.data_ptr() if top else None, self._stream()))
+        return LogProbs(lp, entropy, ids, best)
 
     def matmul_moe(self, x, w: Q4KWeight, n_rows_per_expert: int, offsets, x_rows=None, bias=None, out=None):
         """Indirect form: slot s uses weight rows offsets[s] .. offsets[s]+N of the expert stack."""

@@ -433,6 +433,55 @@ int bpq4k_matmul_fused_f32(bpq4k_handle_t h, int qtype, int prologue, const floa
  * pointers.  Calls on one handle that may overlap on the GPU must be serialised by the caller. */
 int bpq4k_argmax_f32(bpq4k_handle_t h, const float* logits, uint32_t n, int32_t* result, void* stream);
 
+/* ---- the 8-bit path: norm, product, answer -------------------------------------
+ * Rows of 8-bit codes with one float scale per row (a token's activations, an output channel's weights), the operator that
+ * makes them from the residual stream, the product of two such matrices, and what is read off the logits.  The reference has an
+ * 8-bit path of its own (Q8_0 blocks of 32, to which it re-quantises files that are not uniformly K-quant,
+ * runtime/model_runner.cpp:1014-1049, with its residual addition and norm as one dispatch ahead of each projection); one scale per
+ * row lets the whole product run in integers.
+ * Element types of activations and logits are GGUF's numbers (runtime/gguf_loader.h:27-30).  Strides (ld...) are distances
+ * between rows in elements, at least the row's length.  Rows of codes begin at multiples of 16 bytes and can be read to the next
+ * multiple of 16 behind their K codes (the last row too); what lies there may be anything and is not written.
+ * These calls allocate nothing, keep nothing and share nothing: they may be captured without a warm-up call, and calls on
+ * different streams may overlap.  M = 0 does nothing.  Outputs may not overlap inputs except where it is said. */
+enum bpq4k_ftype { BPQ4K_TYPE_F32 = 0, BPQ4K_TYPE_F16 = 1, BPQ4K_TYPE_BF16 = 30 };
+
+/* Residual addition, root-mean-square norm, quantisation; for every row m:
+ *     v = X + residual                    in float; residual may be NULL
+ *     sum = v                             rounded to the element type; may be NULL, may be X or residual themselves
+ *     p = v * weight,  a = max |p|
+ *     codes = round(127 p / a)            to the nearest, ties to the even code: the exact quotient, whatever the order of sums
+ *     scales = a / sqrt(mean(v^2) + eps) / 127
+ * so that codes * scales is the norm's output.  A row of zeros has codes and scale 0.  A row in which a value or a product is
+ * infinite or not a number has codes 0 and a NaN as its scale, which reaches everything that is made of it.  1 <= K <= 32768.
+ * Replaces add_rms_norm and the activation side of the Q8 dispatches (runtime/model_runner.cpp:3200-3243). */
+int bpq4k_add_rmsnorm_i8(bpq4k_handle_t h, int ftype, const void* X, const void* residual, const float* weight, float eps,
+                         void* sum, int8_t* codes, float* scales, uint32_t M, uint32_t K, uint32_t ldx, uint32_t ldr,
+                         uint32_t lds, uint32_t ldc, void* stream);
+
+/* The quantisation alone: codes = round(127 X / a), scales = a / 127, a = max |X| of the row.  For the inputs of projections
+ * that follow no norm, and for weights at load time (a row per output channel). */
+int bpq4k_quantize_i8(bpq4k_handle_t h, int ftype, const void* X, int8_t* codes, float* scales, uint32_t M, uint32_t K,
+                      uint32_t ldx, uint32_t ldc, void* stream);
+
+/* Y[m*ldy + n] = (sum_k X[m][k] * W[n][k]) * x_scales[m] * w_scales[n] + bias[n], of type ftype; bias may be NULL.  The sum is
+ * an exact integer, rounded to float once, so the result does not depend on which kernel serves the call.  1 <= K <= 131071 (the sum of
+ * any codes fits 32 bits), M and N up to 2^24.  X and W 16-byte aligned. */
+int bpq4k_matmul_i8(bpq4k_handle_t h, int ftype, const int8_t* X, const float* x_scales, const int8_t* W, const float* w_scales,
+                    const float* bias, void* Y, uint32_t M, uint32_t N, uint32_t K, uint32_t ldx, uint32_t ldw, uint32_t ldy,
+                    void* stream);
+
+/* What M rows of V logits say, in one pass over them; beside bpq4k_argmax_f32.
+ *     given_lp[m][g] = log softmax(logits[m])[given[m][g]]        nGiven tokens a row (0: given and given_lp are not read);
+ *                                                                 an id outside 0 .. V-1 gives a NaN
+ *     entropy[m] = - sum p log p, in nats                         may be NULL
+ *     top_ids[m][i], top_lp[m][i]                                 the nTop most likely tokens, descending, the lowest index first
+ *                                                                 among equal ones; nTop <= 32 and <= V (0: not written)
+ * Logits of -infinity are tokens of probability 0 (a mask); they come last among the alternatives.  A row that has nothing else: log
+ * probabilities -infinity, entropy 0.  A row with a NaN or +infinity: NaNs, and -1 as ids. */
+int bpq4k_logprobs(bpq4k_handle_t h, int ftype, const void* logits, uint32_t M, uint32_t V, uint32_t ld, const int32_t* given,
+                   uint32_t nGiven, float* given_lp, float* entropy, uint32_t nTop, int32_t* top_ids, float* top_lp, void* stream);
+
 /* ---- GGUF files ------------------------------------------------------------
  * Reader for the file format the weights come in, and the tensor -> device step.  Stands in for
  * GGUFFile::open and its accessors (runtime/gguf_loader.h:46-91, runtime/gguf_loader.cpp:14-182)
