@@ -1,6 +1,19 @@
 // Matrix product of 8-bit rows with 8-bit weights: Y[m][n] = (sum_k x[m][k] * w[n][k]) * xs[m] * ws[n] + bias[n].
 //
-// The sum is an exact 32-bit integer (K <= 131071), so no order of it changes a bit of the result.
+// The sum is an exact 32-bit integer (K <= 131071), so neither the order of it nor the split of K changes a bit of the result.
+//
+// tcgen05.mma.kind::i8 with the weights as the M side (128 rows of a CTA, 256 of a pair) and up to 256 activation rows as the N
+// side: one lane of tensor memory is one output channel, so a warp's store of one activation row is 32 neighbouring outputs.
+// Both operands come by TMA in steps of 128 codes (128-byte swizzle); rows behind M, N and codes behind K arrive as zeros.
+//   one CTA    few activation rows.  Bound by reading the weights; CTAs of a cluster share the K range of a tile where there
+//              are fewer tiles than SMs, and each adds up and stores its share of the tile's columns.
+//   a pair     many activation rows (tcgen05 cta_group::2): each CTA loads half of either operand.
+// Roles (12 warps): warp 0 TMA, warp 1 mma, warp 2 tensor memory, warps 4-11 epilogue.  Persistent over the tiles; two
+// accumulators, so that a tile accumulates while the one before it is stored.
+//
+// Every wait is bounded: on a time-out the role raises the CTA's abort flag and the device status word, waits return at once
+// from then on, copies and mmas in flight are waited for (bounded too), and all threads meet at the end.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -20,62 +33,397 @@ __device__ __forceinline__ __half to_elem<__half>(float v) { return __float2half
 template <>
 __device__ __forceinline__ __nv_bfloat16 to_elem<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// 16 codes from byte k of a row on, zeros from byte K on (the bytes behind a row's codes may be anything).
-__device__ __forceinline__ int4 codes16(const int8_t* row, uint32_t k, uint32_t K) {
-    int4 v = __ldg(reinterpret_cast<const int4*>(row + k));
-    if (k + 16u > K) {
-        const uint32_t n = K - k;  // 1..15 codes
-        auto keep = [n](int w, uint32_t first) { return n >= first + 4u ? w : n <= first ? 0 : w & (int)((1u << (8u * (n - first))) - 1u); };
-        v.x = keep(v.x, 0), v.y = keep(v.y, 4), v.z = keep(v.z, 8), v.w = keep(v.w, 12);
+// The same three roundings in every kernel: the sum to a float, its product with xs, and that times ws plus the bias.
+__device__ __forceinline__ float finish(int s, float xs, float ws, float bias) { return fmaf(__fmul_rn((float)s, xs), ws, bias); }
+
+// ---- tensor cores -------------------------------------------------------------------------------------------------------
+
+constexpr uint32_t kWaitLimit = 1u << 21;
+constexpr uint32_t kSuspendNs = 1000;
+constexpr uint32_t kStep = 128;                       // codes of a row per ring stage: the swizzle's row
+constexpr uint32_t kEpilogueWarps = 8, kThreads = (4 + kEpilogueWarps) * 32;
+constexpr uint32_t kMaxStages = 12;
+constexpr uint32_t kMaxTile = 256;                    // activation rows of a tile
+
+struct TcArgs {
+    CUtensorMap tmap_w, tmap_x;  // [rows][K] bytes, boxes of 128 codes x 128 weight rows | tile / CTAs of the pair activation rows
+    const float* xs;
+    const float* ws;
+    const float* bias;
+    void* Y;
+    uint32_t M, N, ldy;
+    uint32_t tile, m_tiles, tiles, chunks;  // activation rows of a tile, tiles along M, tiles in all, steps along K
+    uint32_t splits;                        // CTAs that share a tile's K range (one CTA form)
+    uint32_t stages, tmem_cols;
+    int* status;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint32_t mbar_try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(kSuspendNs)
+        : "memory");
+    return ok;
+}
+// Bounded wait; false once the CTA is aborting (then at once: the caller carries on so that barriers stay matched).
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status) {
+    if (mbar_try_wait(bar, parity)) return true;
+    for (uint32_t i = 0; i < kWaitLimit; i++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 63u) == 0u && *abort_flag) return false;
     }
-    return v;
+    *abort_flag = 1;
+    if (status) atomicExch(status, kDeviceTimeout);
+    return false;
+}
+// The same for what is still in flight at the end: also waits while the CTA aborts.
+__device__ __forceinline__ void wait_in_flight(uint32_t bar, uint32_t parity) {
+    for (uint32_t i = 0; i < kWaitLimit; i++)
+        if (mbar_try_wait(bar, parity)) return;
+}
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A tile load into this CTA; its completion is counted on `bar`, for a pair on the leader's (a cluster address).
+template <int CG>
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* tmap, uint32_t x, uint32_t y, uint32_t bar) {
+    if constexpr (CG == 1)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+            "l"(tmap), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+            "l"(tmap), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+}
+// K-major shared-memory descriptor, version 1 (sm_100): rows of 128 B, 128-byte swizzle, 8-row groups 1024 B apart.
+__device__ __forceinline__ uint64_t desc_128(uint32_t a) { return (uint64_t)((a >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61); }
+template <int CG>
+__device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (CG == 1)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+            "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+            "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+// Arrives on the barrier (of a pair: at this offset in both CTAs) when the mmas issued so far are done.
+template <int CG>
+__device__ __forceinline__ void umma_commit(uint32_t bar) {
+    if constexpr (CG == 1) {
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    } else {
+        const uint16_t both = 3;
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(both)
+                     : "memory");
+    }
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+                   "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueWarps * 32) : "memory"); }
+
+// Shared memory behind the ring: activation scales of two tiles, barriers, flags; the exchange of a shared tile.
+constexpr uint32_t kScaleBytes = 2u * kMaxTile * 4u, kBarBytes = 512u;
+constexpr uint32_t stage_bytes(uint32_t tile, uint32_t cg) { return 128u * kStep + tile / cg * kStep; }
+constexpr uint32_t exchange_bytes(uint32_t tile, uint32_t splits) { return splits > 1u ? tile * 128u * 4u : 0u; }
+constexpr uint32_t smem_bytes(uint32_t stages, uint32_t tile, uint32_t cg, uint32_t splits) {
+    return 1024u + stages * stage_bytes(tile, cg) + kScaleBytes + kBarBytes + exchange_bytes(tile, splits);
 }
 
-// One warp per weight row, MT activation rows at a time.
-template <typename T, int MT>
-__global__ void __launch_bounds__(256) matmul_i8_dot_kernel(const __grid_constant__ MatmulI8Args a) {
-    const uint32_t n = blockIdx.x * 8u + (threadIdx.x >> 5), lane = threadIdx.x & 31u, m0 = blockIdx.y * MT;
-    if (n >= a.N) return;
-    const int8_t* w = a.W + (uint64_t)n * a.ldw;
-    int acc[MT];
-#pragma unroll
-    for (int i = 0; i < MT; i++) acc[i] = 0;
-    for (uint32_t k = lane * 16u; k < a.K; k += 512u) {
-        const int4 wv = codes16(w, k, a.K);
-#pragma unroll
-        for (int i = 0; i < MT; i++) {
-            if (m0 + i >= a.M) break;
-            const int4 xv = codes16(a.X + (uint64_t)(m0 + i) * a.ldx, k, a.K);
-            acc[i] = __dp4a(xv.x, wv.x, __dp4a(xv.y, wv.y, __dp4a(xv.z, wv.z, __dp4a(xv.w, wv.w, acc[i]))));
+template <int CG, typename T>
+__global__ void __launch_bounds__(kThreads, 2) matmul_i8_kernel(const __grid_constant__ TcArgs a) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t sbytes = stage_bytes(a.tile, CG), off_scale = a.stages * sbytes, off_bar = off_scale + kScaleBytes;
+    float* scale = reinterpret_cast<float*>(base_ptr + off_scale);
+    const uint32_t bar0 = base + off_bar, exchange = bar0 + kBarBytes;
+    auto full = [&](uint32_t s) { return bar0 + s * 8u; };
+    auto empty = [&](uint32_t s) { return bar0 + (kMaxStages + s) * 8u; };
+    auto acc_full = [&](uint32_t b) { return bar0 + (2u * kMaxStages + b) * 8u; };
+    auto acc_empty = [&](uint32_t b) { return bar0 + (2u * kMaxStages + 2u + b) * 8u; };
+    const uint32_t parts_bar = bar0 + (2u * kMaxStages + 4u) * 8u, done_bar = parts_bar + 8u;
+    static_assert((2u * kMaxStages + 8u) * 8u <= kBarBytes, "barrier area");
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + off_bar + (2u * kMaxStages + 6u) * 8u);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + off_bar + (2u * kMaxStages + 6u) * 8u + 4u);
+
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    uint32_t rank = 0;
+    if (CG == 2 || a.splits > 1u) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const uint32_t group = CG == 2 ? 2u : a.splits;            // CTAs of a cluster
+    const uint32_t first_tile = blockIdx.x / group, step_tile = gridDim.x / group;
+    const uint32_t half = CG == 2 ? rank : 0u;                 // which half of the pair's operands
+    const bool leader = CG == 1 || rank == 0u;
+    const uint32_t c0 = CG == 2 ? 0u : (uint32_t)((uint64_t)a.chunks * rank / a.splits);
+    const uint32_t c1 = CG == 2 ? a.chunks : (uint32_t)((uint64_t)a.chunks * (rank + 1u) / a.splits);
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < a.stages; s++) mbar_init(full(s), 1), mbar_init(empty(s), 1);
+        for (uint32_t b = 0; b < 2; b++) mbar_init(acc_full(b), 1), mbar_init(acc_empty(b), CG * kEpilogueWarps);
+        mbar_init(parts_bar, group * kEpilogueWarps);
+        mbar_init(done_bar, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 2) {
+        if constexpr (CG == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(a.tmem_cols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(a.tmem_cols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
         }
     }
+    fence_before();
+    if (group > 1u) cluster_sync_all();  // barriers and tensor memory are ready before anything crosses over
+    else __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // all that is read comes from earlier kernels
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---------------- operands ----------------
+            uint32_t s = 0, it = 0, issued = 0;
+            const uint32_t full0 = CG == 2 ? peer_addr(full(0), 0u) : full(0);
+            bool ok = true;
+            for (uint32_t t = first_tile; t < a.tiles && ok; t += step_tile) {
+                const uint32_t rt = t / a.m_tiles, n0 = (rt * CG + half) * 128u, m0 = (t - rt * a.m_tiles) * a.tile + half * (a.tile / CG);
+                for (uint32_t c = c0; c < c1; c++) {
+                    ok = it == 0 || wait_bar(empty(s), (it - 1u) & 1u, abort_flag, a.status);
+                    if (!ok) break;
+                    const uint32_t dst = base + s * sbytes, bar = full0 + s * 8u;
+                    if (!BPQ4K_CHECK(s < a.stages && c < a.chunks && rt * CG * 128u < a.N, a.status)) {
+                        *abort_flag = 1, ok = false;
+                        break;
+                    }
+                    if (leader) mbar_expect_tx(full(s), CG * sbytes);
+                    tma_load<CG>(dst, &a.tmap_w, c * kStep, n0, bar);
+                    tma_load<CG>(dst + 128u * kStep, &a.tmap_x, c * kStep, m0, bar);
+                    issued++;
+                    if (++s == a.stages) s = 0, it++;
+                }
+            }
+            if (!ok && leader)  // aborting: nothing may still be written to shared memory after the exit
+                for (uint32_t i = issued > a.stages ? issued - a.stages : 0u; i < issued; i++) wait_in_flight(full(i % a.stages), (i / a.stages) & 1u);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            // ---------------- products ----------------
+            const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((a.tile >> 3) << 17) | ((CG * 128u >> 4) << 24);  // s32 += s8 * s8, K-major
+            uint32_t s = 0, it = 0, i = 0;
+            bool ok = true;
+            for (uint32_t t = first_tile; t < a.tiles && ok; t += step_tile, i++) {
+                const uint32_t buf = i & 1u, d = tmem + buf * a.tile;
+                ok = i < 2u || wait_bar(acc_empty(buf), ((i >> 1) - 1u) & 1u, abort_flag, a.status);
+                fence_after();
+                for (uint32_t c = c0; c < c1 && ok; c++) {
+                    ok = wait_bar(full(s), it & 1u, abort_flag, a.status);
+                    if (!ok) break;
+                    fence_after();
+                    const uint64_t da = desc_128(base + s * sbytes), db = desc_128(base + s * sbytes + 128u * kStep);
 #pragma unroll
-    for (int i = 0; i < MT; i++) {
-        const int s = __reduce_add_sync(0xFFFFFFFFu, acc[i]);
-        if (lane == (uint32_t)i && m0 + i < a.M) {
-            float y = (float)s * a.xs[m0 + i] * a.ws[n];
-            if (a.bias) y += a.bias[n];
-            static_cast<T*>(a.Y)[(uint64_t)(m0 + i) * a.ldy + n] = to_elem<T>(y);
+                    for (uint32_t k = 0; k < kStep / 32u; k++) umma<CG>(d, da + k * 2u, db + k * 2u, idesc, (c > c0 || k) ? 1u : 0u);
+                    umma_commit<CG>(empty(s));
+                    if (++s == a.stages) s = 0, it++;
+                }
+                if (ok) umma_commit<CG>(acc_full(buf));
+            }
+            if (!ok) {
+                umma_commit<CG>(done_bar);
+                wait_in_flight(done_bar, 0u);
+            }
+        }
+    } else if (warp >= 4) {
+        // ---------------- epilogue ----------------
+        const uint32_t e = threadIdx.x - 128u, quad = warp & 3u, side = (warp - 4u) >> 2, r = quad * 32u + lane;
+        T* Y = static_cast<T*>(a.Y);
+        uint32_t i = 0;
+        for (uint32_t t = first_tile; t < a.tiles; t += step_tile, i++) {
+            const uint32_t rt = t / a.m_tiles, n = (rt * CG + half) * 128u + r, m0 = (t - rt * a.m_tiles) * a.tile, buf = i & 1u;
+            const uint32_t cols = min(a.tile, a.M - m0);
+            const bool live = n < a.N;
+            const float wscale = live ? __ldg(a.ws + n) : 0.f, bias = live && a.bias ? __ldg(a.bias + n) : 0.f;
+            float* xscale = scale + buf * kMaxTile;
+            if (e < cols) xscale[e] = __ldg(a.xs + m0 + e);
+            epilogue_sync();
+            const bool ok = wait_bar(acc_full(buf), (i >> 1) & 1u, abort_flag, a.status);
+            fence_after();
+            const uint32_t acc = tmem + ((quad * 32u) << 16) + buf * a.tile;
+            if (CG == 2 || a.splits == 1u) {
+                for (uint32_t c = side * 16u; c < cols && ok; c += 32u) {
+                    uint32_t v[16];
+                    tmem_ld16(acc + c, v);
+                    T* y = Y + (uint64_t)(m0 + c) * a.ldy + n;
+                    if (live) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 16; j++)
+                            if (c + j < cols) y[(uint64_t)j * a.ldy] = to_elem<T>(finish((int)v[j], xscale[c + j], wscale, bias));
+                    }
+                }
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(peer_addr(acc_empty(buf), CG == 2 ? 0u : rank));
+            } else {
+                // every CTA of the cluster has a part of each sum: CTA q adds up and stores the q-th share of the columns
+                const uint32_t share = a.tile / a.splits;
+                for (uint32_t c = side * 16u; c < cols && ok; c += 32u) {
+                    uint32_t v[16];
+                    tmem_ld16(acc + c, v);
+#pragma unroll
+                    for (uint32_t j = 0; j < 16; j++) {
+                        const uint32_t q = (c + j) / share;
+                        if (c + j < cols)
+                            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_addr(exchange, q) + ((rank * share + (c + j) - q * share) * 128u + r) * 4u),
+                                         "r"(v[j])
+                                         : "memory");
+                    }
+                }
+                asm volatile("fence.acq_rel.cluster;" ::: "memory");
+                __syncwarp();
+                if (lane == 0)
+                    for (uint32_t q = 0; q < a.splits; q++) mbar_arrive_cluster(peer_addr(parts_bar, q));
+                const bool all = wait_bar(parts_bar, 0u, abort_flag, a.status);
+                const int* parts = reinterpret_cast<const int*>(base_ptr + off_bar + kBarBytes);
+                for (uint32_t c = side; c < share && rank * share + c < cols && all && live; c += 2u) {
+                    int sum = 0;
+                    for (uint32_t p = 0; p < a.splits; p++) sum += parts[(p * share + c) * 128u + r];
+                    const uint32_t m = rank * share + c;
+                    Y[(uint64_t)(m0 + m) * a.ldy + n] = to_elem<T>(finish(sum, xscale[m], wscale, bias));
+                }
+            }
         }
     }
+    __syncwarp();
+    fence_before();
+    if (group > 1u) cluster_sync_all();  // nothing crosses over any more
+    else __syncthreads();
+    if (warp == 2) {
+        fence_after();
+        if constexpr (CG == 1)
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
+    }
+}
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+    static EncodeTiledFn fn = []() -> EncodeTiledFn {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+            return nullptr;
+        return reinterpret_cast<EncodeTiledFn>(p);
+    }();
+    return fn;
+}
+bool encode_rows(CUtensorMap* map, const int8_t* codes, uint32_t rows, uint32_t K, uint32_t ld, uint32_t box_rows) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return false;
+    const cuuint64_t gdim[2] = {K, rows}, gstride[1] = {ld};
+    const cuuint32_t box[2] = {kStep, box_rows}, estr[2] = {1u, 1u};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(codes), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int CG, typename T>
+cudaError_t launch_tc(const MatmulI8Args& m, int* status_dev, int sm_count, cudaStream_t stream) {
+    TcArgs a{};
+    a.xs = m.xs, a.ws = m.ws, a.bias = m.bias, a.Y = m.Y, a.M = m.M, a.N = m.N, a.ldy = m.ldy, a.status = status_dev;
+    const uint32_t unit = CG * 16u;  // the mma's step of N
+    a.m_tiles = (m.M + kMaxTile - 1u) / kMaxTile;
+    a.tile = ((m.M + a.m_tiles - 1u) / a.m_tiles + unit - 1u) / unit * unit;
+    a.m_tiles = (m.M + a.tile - 1u) / a.tile;
+    a.chunks = (m.K + kStep - 1u) / kStep;
+    const uint64_t tiles = (uint64_t)((m.N + CG * 128u - 1u) / (CG * 128u)) * a.m_tiles;
+    if (tiles > 0x7FFFFFFFull) return cudaErrorInvalidValue;
+    a.tiles = (uint32_t)tiles;
+    a.splits = 1;
+    if (CG == 1)  // few tiles: up to eight CTAs share the K range of one
+        while (a.splits < 8u && a.tile <= 64u && a.tiles * a.splits * 2u <= 2u * (uint32_t)sm_count && a.chunks >= a.splits * 4u) a.splits *= 2u;
+    const uint32_t group = CG == 2 ? 2u : a.splits;
+    const uint32_t budget = a.splits > 1u ? 112u * 1024u : 226u * 1024u;
+    a.stages = (budget - smem_bytes(0, a.tile, CG, a.splits)) / stage_bytes(a.tile, CG);
+    if (a.stages > kMaxStages) a.stages = kMaxStages;
+    a.tmem_cols = 32;
+    while (a.tmem_cols < (a.splits > 1u ? 1u : 2u) * a.tile) a.tmem_cols *= 2u;
+    uint32_t groups = (uint32_t)sm_count / group;
+    if (a.splits > 1u || groups > a.tiles) groups = a.tiles;
+    if (!encode_rows(&a.tmap_w, m.W, m.N, m.K, m.ldw, 128u) || !encode_rows(&a.tmap_x, m.X, m.M, m.K, m.ldx, a.tile / CG)) return cudaErrorInvalidValue;
+    const uint32_t smem = smem_bytes(a.stages, a.tile, CG, a.splits);
+    static KernelConfig kcfg;
+    if (cudaError_t e = kcfg.prepare(reinterpret_cast<const void*>(matmul_i8_kernel<CG, T>), kThreads, smem, nullptr)) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(groups * group);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = group, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = group > 1u ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, matmul_i8_kernel<CG, T>, a);
 }
 
 template <typename T>
-cudaError_t launch_type(const MatmulI8Args& a, cudaStream_t stream) {
-    matmul_i8_dot_kernel<T, 8><<<dim3((a.N + 7u) / 8u, (a.M + 7u) / 8u), 256, 0, stream>>>(a);
-    return cudaGetLastError();
+cudaError_t launch_type(const MatmulI8Args& a, int* status_dev, int sm_count, cudaStream_t stream) {
+    return a.M <= 64u ? launch_tc<1, T>(a, status_dev, sm_count, stream) : launch_tc<2, T>(a, status_dev, sm_count, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_matmul_i8(const MatmulI8Args& a, int ftype, int* status_dev, int sm_count, cudaStream_t stream, int* launches) {
-    (void)status_dev, (void)sm_count;
     if (a.M == 0 || a.N == 0) return cudaSuccess;
     ++*launches;
     switch (ftype) {
-        case 0: return launch_type<float>(a, stream);
-        case 1: return launch_type<__half>(a, stream);
-        case 30: return launch_type<__nv_bfloat16>(a, stream);
+        case 0: return launch_type<float>(a, status_dev, sm_count, stream);
+        case 1: return launch_type<__half>(a, status_dev, sm_count, stream);
+        case 30: return launch_type<__nv_bfloat16>(a, status_dev, sm_count, stream);
         default: return cudaErrorInvalidValue;
     }
 }
