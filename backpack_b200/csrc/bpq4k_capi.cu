@@ -1136,8 +1136,8 @@ int bpq4k_logprobs(bpq4k_handle_t h, int ftype, const void* logits, uint32_t M, 
     DeviceGuard g(h->device);
     LogprobsArgs a{};
     a.logits = logits, a.given = given, a.given_lp = given_lp, a.entropy = entropy, a.top_ids = top_ids, a.top_lp = top_lp;
-    a.M = M, a.V = V, a.ld = ld, a.nGiven = nGiven, a.nTop = nTop;
-    const cudaError_t e = launch_logprobs(a, ftype, static_cast<cudaStream_t>(stream));
+    a.M = M, a.V = V, a.ld = ld, a.nGiven = nGiven, a.nTop = nTop, a.status = h->dev_status;
+    const cudaError_t e = launch_logprobs(a, ftype, h->sm_count, static_cast<cudaStream_t>(stream));
     h->launches += 1;
     if (e != cudaSuccess) return cuda_fail(h, e, "log probability launch");
     return BPQ4K_OK;

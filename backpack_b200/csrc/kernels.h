@@ -203,8 +203,9 @@ struct LogprobsArgs {
     int32_t* top_ids;      // [M][nTop]
     float* top_lp;         // [M][nTop]
     uint32_t M, V, ld, nGiven, nTop;
+    int* status;           // debug build
 };
-cudaError_t launch_logprobs(const LogprobsArgs& a, int ftype, cudaStream_t stream);
+cudaError_t launch_logprobs(const LogprobsArgs& a, int ftype, int sm_count, cudaStream_t stream);
 
 // Cross-GPU barrier on flag words in peer memory (one process per GPU): store `epoch` into slot
 // `rank` of every peer's flag array, then wait -- at most timeout_cycles -- until every slot of the

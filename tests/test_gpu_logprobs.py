@@ -162,9 +162,14 @@ def test_rows_without_a_distribution(ctx):
         got = ctx.logprobs(x, given=given, top=3)
         for r in (1, 2, 3):
             assert torch.isnan(got.given[r]).all() and torch.isnan(got.entropy[r]) and torch.isnan(got.top[r]).all() and (got.top_ids[r] == -1).all()
+        # the other rows are as they are by themselves.  Which values a thread adds up follows from the row's place between
+        # 16-byte boundaries (row 1 of two begins elsewhere than row 4 of five), so each result is within its own bound of the
+        # exact value, and the two within twice that of each other
         rest = ctx.logprobs(x[::4].contiguous(), given=given[::4].contiguous(), top=3)
-        for a, b in ((got.given, rest.given), (got.entropy, rest.entropy), (got.top, rest.top), (got.top_ids, rest.top_ids)):
-            assert torch.equal(a[::4], b)
+        assert torch.equal(got.top_ids[::4], rest.top_ids)
+        for a, b, n in ((got.given, rest.given, 1), (got.entropy, rest.entropy, 3), (got.top, rest.top, 1)):
+            bound = n * (V / 512 + 80) * U
+            assert bool(((a[::4] - b).abs() <= 2 * (bound + (bound if n == 3 else 4 * U) * b.abs())).all())
 
 
 def test_given_tokens_outside_the_row(ctx):
