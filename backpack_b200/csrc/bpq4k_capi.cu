@@ -1055,7 +1055,7 @@ int rows_i8(bpq4k_context* h, int ftype, const RowsI8Args& a, cudaStream_t st) {
     if (int s = check_codes(h, "codes", a.codes, a.K, a.ldc)) return s;
     if (int s = check_floats(h, "scales", a.scales)) return s;
     DeviceGuard g(h->device);
-    const cudaError_t e = launch_rows_i8(a, ftype, st);
+    const cudaError_t e = launch_rows_i8(a, ftype, h->sm_count, st);
     h->launches += 1;
     if (e != cudaSuccess) return cuda_fail(h, e, "8-bit rows launch");
     return BPQ4K_OK;

@@ -5,13 +5,16 @@
 //   code = round_half_even(127 p / a),   scale = a * rstd / 127
 // rstd is a factor of the whole row and of its largest value, so the codes do not depend on it: they are computed from the
 // exact quotient and never differ with the order of a sum.  In float the quotient is off by at most 127 * 3 * 2^-24 = 2.3e-5
-// (the product, 127/a and their product are rounded); a quotient that lies nearer than 4e-5 to the middle between two codes
-// is computed again in double from the exact product (48 bits) and the exact a.
+// (the product, a and 127/a are rounded; the quotient's distance from its code is not, it is a multiply-add).  Where one lies
+// nearer than 3e-5 to the middle between two codes, its code is computed again in double, from the exact product (48 bits) and
+// the exact a.
 //
 // Memory bound (13 bytes a value with a float residual stream).  A row's values stay in registers between the two halves
-// (statistics, codes); the reduction in between takes one barrier.
+// (statistics, codes), one CTA to a row, several rows to an SM, so that one row's loads overlap another's arithmetic.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "kernels.h"
 #include "q4k_common.cuh"
@@ -20,23 +23,9 @@ namespace bpq4k {
 
 namespace {
 
-template <typename T>
-struct Elem;
-template <>
-struct Elem<float> {
-    static __device__ __forceinline__ float get(float v) { return v; }
-    static __device__ __forceinline__ float put(float v) { return v; }
-};
-template <>
-struct Elem<__half> {
-    static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
-    static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
-};
-template <>
-struct Elem<__nv_bfloat16> {
-    static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
-    static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
-};
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
 // E elements with one access: 16 bytes, or a single element on rows that are not 16-byte aligned.
 template <typename T, int E>
@@ -54,22 +43,62 @@ __device__ __forceinline__ Pack<T, E> load_pack(const T* p) {
     }
     return r;
 }
+// E floats, rounded to the element type (two at a time: a single conversion to 16 bits has a sixteenth of the rate).
 template <typename T, int E>
-__device__ __forceinline__ void store_pack(T* p, const Pack<T, E>& r) {
-    if constexpr (E == 1)
-        *p = r.v[0];
-    else
-        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(r.v);
+__device__ __forceinline__ void store_pack(T* p, const float* v) {
+    if constexpr (sizeof(T) == 4 && E == 1) {
+        *p = v[0];
+    } else if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        T2 w[(E + 1) / 2];
+#pragma unroll
+        for (int j = 0; j < E; j += 2) {
+            const float second = E == 1 ? 0.f : v[j + (E > 1)];
+            if constexpr (std::is_same<T, __half>::value)
+                w[j / 2] = __floats2half2_rn(v[j], second);
+            else
+                w[j / 2] = __floats2bfloat162_rn(v[j], second);
+        }
+        if constexpr (E == 1)
+            *p = w[0].x;
+        else
+            *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(w);
+    }
 }
 
-// Monotonic map of a float to an unsigned word, and back.
-__device__ __forceinline__ uint32_t ordered(float f) {
-    const uint32_t b = __float_as_uint(f);
-    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+__device__ __forceinline__ float max_nan(float a, float b) {  // a NaN if either is one
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
-__device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u); }
 
-// A thread holds PT values: PT / E accesses, blockDim.x of them apart.
+constexpr float kNear = 0.5f - 3e-5f;  // a quotient further from its code than this may belong to the next one
+
+// The code of 127 p / peak, which lies in [k, k + 1): on which side of k + 1/2 it is.
+__device__ __forceinline__ uint32_t exact_code(double p, double peak, int k) {
+    const double l = 254.0 * p, r = (double)(2 * k + 1) * peak;
+    return (uint32_t)(l < r || (l == r && (k & 1) == 0) ? k : k + 1);
+}
+
+template <int E>
+__device__ __forceinline__ void store_codes(int8_t* at, const uint32_t (&q)[E]) {
+    if constexpr (E == 1) {
+        *at = (int8_t)(q[0] & 0xFFu);
+    } else {
+        uint32_t w[E / 4];
+#pragma unroll
+        for (int j = 0; j < E; j += 4)
+            w[j / 4] = __byte_perm(__byte_perm(q[j], q[j + 1], 0x0040), __byte_perm(q[j + 2], q[j + 3], 0x0040), 0x5410);
+        if constexpr (E == 4)
+            *reinterpret_cast<uint32_t*>(at) = w[0];
+        else
+            *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+    }
+}
+
+// A thread holds PT values: PT / E accesses, blockDim.x of them apart; as they were loaded, or (RES) their sums in float.
 template <typename T, int E, int PT, bool NORM, bool RES>
 __global__ void __launch_bounds__(1024) rows_i8_kernel(const __grid_constant__ RowsI8Args a) {
     constexpr int NV = PT / E;
@@ -91,11 +120,12 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(const __grid_constant__ R
         }
     };
 
-    float v[PT];
-    float ss = 0.f, lo = 0.f;
-    uint32_t hi = 0u;  // the largest |p| as bits: a NaN or an infinity is the largest of all; `lo` its exact rounding error
+    Pack<T, E> xv[NV] = {};
+    float v[RES ? PT : 1] = {};
+    auto value = [&](int i, int j) { return RES ? v[RES ? i * E + j : 0] : to_float(xv[i].v[j]); };
+    float ss = 0.f, hi = 0.f;  // (an infinity or a NaN reaches hi)
     {
-        Pack<T, E> xv[NV], rv[RES ? NV : 1];
+        Pack<T, E> rv[RES ? NV : 1];
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const uint32_t e = (tid + i * blockDim.x) * E;
@@ -111,69 +141,47 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(const __grid_constant__ R
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const uint32_t e = (tid + i * blockDim.x) * E;
-            if (e >= a.K) {
-#pragma unroll
-                for (int j = 0; j < E; j++) v[i * E + j] = 0.f;
-                continue;
-            }
+            if (e >= a.K) continue;
             float w[E];
             if constexpr (NORM) weights(e, w);
 #pragma unroll
             for (int j = 0; j < E; j++) {
-                float s = Elem<T>::get(xv[i].v[j]);
-                if constexpr (RES) s += Elem<T>::get(rv[i].v[j]);
-                v[i * E + j] = s;
-                if constexpr (NORM) {
-                    ss = fmaf(s, s, ss);
-                    const float p = fabsf(s * w[j]);
-                    const uint32_t b = __float_as_uint(p);
-                    if (b >= hi) {
-                        const float l = fmaf(fabsf(s), fabsf(w[j]), -p);
-                        lo = b > hi ? l : fmaxf(lo, l);
-                        hi = b;
-                    }
-                } else {
-                    hi = max(hi, __float_as_uint(fabsf(s)));
-                }
+                if constexpr (RES) v[i * E + j] = to_float(xv[i].v[j]) + to_float(rv[i].v[j]);
+                const float s = value(i, j);
+                if constexpr (NORM) ss = fmaf(s, s, ss);
+                hi = max_nan(hi, fabsf(NORM ? s * w[j] : s));
             }
-            if (RES && sum) {
-                Pack<T, E> o;
-#pragma unroll
-                for (int j = 0; j < E; j++) o.v[j] = Elem<T>::put(v[i * E + j]);
-                if (BPQ4K_CHECK(e + E <= a.K, a.status)) store_pack<T, E>(sum + e, o);
-            }
+            if constexpr (RES)
+                if (sum && BPQ4K_CHECK(e + E <= a.K, a.status)) store_pack<T, E>(sum + e, v + i * E);
         }
     }
 
-    __shared__ uint32_t s_hi[32], s_lo[32];
+    __shared__ uint32_t s_hi[32];
     __shared__ float s_ss[32];
     __shared__ double s_sq[32], s_peak[32];
-    // the largest (hi, lo) of lanes: the largest hi, and the largest lo beside it
-    auto largest = [](uint32_t& h, uint32_t& l) {
-        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, h);
-        l = __reduce_max_sync(0xFFFFFFFFu, h == top ? l : 0u);
-        h = top;
-    };
-    uint32_t low = ordered(lo);
-    largest(hi, low);
+    __shared__ unsigned long long s_exact;  // the exact a, as the bits of a double (positive ones order like whole numbers)
+    const uint32_t mine = __float_as_uint(hi);
+    const uint32_t warp_hi = __reduce_max_sync(0xFFFFFFFFu, mine);
     if constexpr (NORM) {
 #pragma unroll
         for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
     }
-    if (lane == 0) s_hi[warp] = hi, s_lo[warp] = low, s_ss[warp] = ss;
+    if (lane == 0) s_hi[warp] = warp_hi, s_ss[warp] = ss;
+    if (tid == 0) s_exact = 0ull;
     __syncthreads();
-    hi = lane < warps ? s_hi[lane] : 0u;
-    low = lane < warps ? s_lo[lane] : 0u;
-    largest(hi, low);
-    double rstd = 1.0, peak = (double)__uint_as_float(hi) + (NORM ? (double)unordered(low) : 0.0);
+    const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, lane < warps ? s_hi[lane] : 0u);
+    const float peak = __uint_as_float(top);
+    const bool bad = !(peak < __uint_as_float(0x7F800000u)), tiny = peak < 1e-30f;  // (tiny: products and 127 / a leave the float range)
+    double largest = (double)peak, sq = 0.0;
     if constexpr (NORM) {
         ss = lane < warps ? s_ss[lane] : 0.f;
 #pragma unroll
         for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-        double sq = ss;
-        // squares, or low parts of products, beyond what a float holds well (every thread sees the same, so all or none come here)
-        if (!(ss > 1e-20f && ss < 1e30f) || __uint_as_float(hi) < 1e-30f) {
-            sq = 0.0, peak = 0.0;
+        sq = ss;
+        // squares or products beyond what a float holds well (every thread sees the same, so all or none come here)
+        if (!(ss > 1e-20f && ss < 1e30f) || tiny) {
+            sq = 0.0;
+            double big = 0.0;
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 const uint32_t e = (tid + i * blockDim.x) * E;
@@ -182,33 +190,58 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(const __grid_constant__ R
                 weights(e, w);
 #pragma unroll
                 for (int j = 0; j < E; j++) {
-                    const double s = (double)v[i * E + j];
+                    const double s = (double)value(i, j);
                     sq += s * s;
-                    peak = fmax(peak, fabs(s * (double)w[j]));
+                    big = fmax(big, fabs(s * (double)w[j]));
                 }
             }
 #pragma unroll
             for (int o = 16; o; o >>= 1) {
                 sq += __shfl_xor_sync(0xFFFFFFFFu, sq, o);
-                peak = fmax(peak, __shfl_xor_sync(0xFFFFFFFFu, peak, o));
+                big = fmax(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
             }
-            if (lane == 0) s_sq[warp] = sq, s_peak[warp] = peak;
+            if (lane == 0) s_sq[warp] = sq, s_peak[warp] = big;
             __syncthreads();
             sq = lane < warps ? s_sq[lane] : 0.0;
-            peak = lane < warps ? s_peak[lane] : 0.0;
+            largest = lane < warps ? s_peak[lane] : 0.0;
 #pragma unroll
             for (int o = 16; o; o >>= 1) {
                 sq += __shfl_xor_sync(0xFFFFFFFFu, sq, o);
-                peak = fmax(peak, __shfl_xor_sync(0xFFFFFFFFu, peak, o));
+                largest = fmax(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, o));
             }
         }
-        rstd = rsqrt(sq / (double)a.K + (double)a.eps);
     }
-    const bool bad = hi >= 0x7F800000u;
-    if (tid == 0) a.scales[row] = bad ? __uint_as_float(0x7FC00000u) : peak == 0.0 ? 0.f : (float)(peak * rstd / 127.0);
+    const bool zero = bad || largest == 0.0;
+    if (tid == 0) {
+        const double rstd = NORM ? rsqrt(sq / (double)a.K + (double)a.eps) : 1.0;
+        a.scales[row] = bad ? __uint_as_float(0x7FC00000u) : zero ? 0.f : (float)(largest * rstd / 127.0);
+    }
+    if (zero) {  // (a whole row)
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const uint32_t e = (tid + i * blockDim.x) * E;
+            const uint32_t none[E] = {};
+            if (e < a.K && BPQ4K_CHECK(e + E <= a.K && row < a.M, a.status)) store_codes<E>(codes + e, none);
+        }
+        return;
+    }
 
-    const float inv = 127.f / (float)peak;
-    const bool zero = bad || peak == 0.0, tiny = peak < 1e-30;  // (127 / a, or the low parts of products, leave the float range)
+    // one product, or a few that round to the same float, is the largest: whoever holds it knows a exactly
+    if (NORM && (mine == top || tiny)) {
+        double big = 0.0;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const uint32_t e = (tid + i * blockDim.x) * E;
+            if (e >= a.K) continue;
+            float w[E];
+            weights(e, w);
+#pragma unroll
+            for (int j = 0; j < E; j++) big = fmax(big, fabs((double)value(i, j) * (double)w[j]));
+        }
+        atomicMax(&s_exact, (unsigned long long)__double_as_longlong(big));
+    }
+    const float inv = tiny ? 0.f : 127.f / peak;
+    float far = tiny ? 1.f : 0.f;  // the largest distance of a quotient from its code
 #pragma unroll
     for (int i = 0; i < NV; i++) {
         const uint32_t e = (tid + i * blockDim.x) * E;
@@ -218,30 +251,33 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(const __grid_constant__ R
         uint32_t q[E];
 #pragma unroll
         for (int j = 0; j < E; j++) {
-            const float s = v[i * E + j];
-            const float t = (NORM ? s * w[j] : s) * inv;
-            const float c = t + 12582912.f;  // 1.5 * 2^23: the low byte of the sum is the rounded quotient
+            const float p = NORM ? value(i, j) * w[j] : value(i, j);
+            const float c = fmaf(p, inv, 12582912.f);  // 1.5 * 2^23: the low byte is the rounded quotient
             q[j] = __float_as_uint(c);
-            if (zero) {
-                q[j] = 0u;
-            } else if (tiny || fabsf(t - (c - 12582912.f)) > 0.5f - 4e-5f) {
-                const double p = NORM ? (double)s * (double)w[j] : (double)s;
-                q[j] = (uint32_t)(int32_t)rint(127.0 * p / peak);
-            }
+            far = fmaxf(far, fabsf(fmaf(p, inv, -(c - 12582912.f))));
         }
-        if (!BPQ4K_CHECK(e + E <= a.K && row < a.M, a.status)) continue;
-        if constexpr (E == 1) {
-            codes[e] = (int8_t)(q[0] & 0xFFu);
-        } else {
+        if (BPQ4K_CHECK(e + E <= a.K && row < a.M, a.status)) store_codes<E>(codes + e, q);
+    }
+    if constexpr (NORM) __syncthreads();
+    if (far > kNear) {
+        const double exact = NORM ? __longlong_as_double((long long)s_exact) : (double)peak, by = tiny ? 127.0 / exact : 0.0;
 #pragma unroll
-            for (int j = 0; j < E; j += 4) {
-                const uint32_t word = __byte_perm(__byte_perm(q[j], q[j + 1], 0x0040), __byte_perm(q[j + 2], q[j + 3], 0x0040), 0x5410);
-                q[j / 4] = word;
+        for (int i = 0; i < NV; i++) {
+            const uint32_t e = (tid + i * blockDim.x) * E;
+            if (e >= a.K) continue;
+            float w[E];
+            if constexpr (NORM) weights(e, w);
+            uint32_t q[E];
+#pragma unroll
+            for (int j = 0; j < E; j++) {
+                const float s = value(i, j), p = NORM ? s * w[j] : s, c = fmaf(p, inv, 12582912.f), d = fmaf(p, inv, -(c - 12582912.f));
+                q[j] = __float_as_uint(c);
+                if (tiny || fabsf(d) > kNear) {
+                    const double pp = NORM ? (double)s * (double)w[j] : (double)s;
+                    q[j] = exact_code(pp, exact, tiny ? (int)floor(pp * by) : __float2int_rn(c - 12582912.f) - (d < 0.f ? 1 : 0));
+                }
             }
-            if constexpr (E == 4)
-                *reinterpret_cast<uint32_t*>(codes + e) = q[0];
-            else
-                *reinterpret_cast<uint2*>(codes + e) = make_uint2(q[0], q[1]);
+            if (BPQ4K_CHECK(e + E <= a.K && row < a.M, a.status)) store_codes<E>(codes + e, q);
         }
     }
 }
@@ -258,24 +294,34 @@ cudaError_t launch_pt(const RowsI8Args& a, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
+// Values of a thread.  8: the shortest way through a row, for rows that have an SM each (1 x 4096 float 3.0 us, with 16 3.6), short
+// rows (2048 x 768 float 6.3 against 7.0) and single accesses (2048 x 5001 half 56 against 67).  16: more loads in flight per SM
+// (2048 x 8192 float 38.7 us, with 8 48.3, with 32 53.9; bfloat16 30.1, 39.7, 33.4).  32: rows that need it, and 16-bit rows
+// without a residual from 8192 on, whose values stay packed (512 x 14336 bfloat16 12.5 us, with 16 13.8).
+template <typename T, int E>
+cudaError_t launch_vec(const RowsI8Args& a, int sm_count, cudaStream_t stream) {
+    if (a.K <= 8192u && (a.M <= (uint32_t)sm_count || a.K <= 1024u || E == 1)) return launch_pt<T, E, 8>(a, stream);
+    if (a.K <= 8192u || (a.K <= 16384u && (sizeof(T) == 4 || a.R))) return launch_pt<T, E, 16>(a, stream);
+    return launch_pt<T, E, 32>(a, stream);
+}
+
 template <typename T>
-cudaError_t launch_type(const RowsI8Args& a, cudaStream_t stream) {
+cudaError_t launch_type(const RowsI8Args& a, int sm_count, cudaStream_t stream) {
     constexpr int E = 16 / sizeof(T);
     auto off = [](const void* p, uint32_t ld) { return p && ((reinterpret_cast<uintptr_t>(p) & 15u) || (uint64_t)ld * sizeof(T) % 16u); };
     const bool single = a.K % E || off(a.X, a.ldx) || off(a.R, a.ldr) || off(a.sum, a.lds) || (reinterpret_cast<uintptr_t>(a.w) & 15u);
-    if (single) return a.K <= 8192u ? launch_pt<T, 1, 8>(a, stream) : launch_pt<T, 1, 32>(a, stream);
-    return a.K <= 8192u ? launch_pt<T, E, 8>(a, stream) : launch_pt<T, E, 32>(a, stream);
+    return single ? launch_vec<T, 1>(a, sm_count, stream) : launch_vec<T, E>(a, sm_count, stream);
 }
 
 }  // namespace
 
-cudaError_t launch_rows_i8(const RowsI8Args& a, int ftype, cudaStream_t stream) {
+cudaError_t launch_rows_i8(const RowsI8Args& a, int ftype, int sm_count, cudaStream_t stream) {
     if (a.M == 0) return cudaSuccess;
     if (a.K == 0 || a.K > kRowsI8MaxK || (a.R && !a.w)) return cudaErrorInvalidValue;
     switch (ftype) {
-        case 0: return launch_type<float>(a, stream);
-        case 1: return launch_type<__half>(a, stream);
-        case 30: return launch_type<__nv_bfloat16>(a, stream);
+        case 0: return launch_type<float>(a, sm_count, stream);
+        case 1: return launch_type<__half>(a, sm_count, stream);
+        case 30: return launch_type<__nv_bfloat16>(a, sm_count, stream);
         default: return cudaErrorInvalidValue;
     }
 }

@@ -176,7 +176,7 @@ struct RowsI8Args {
     float eps;
     int* status;        // debug build
 };
-cudaError_t launch_rows_i8(const RowsI8Args& a, int ftype, cudaStream_t stream);
+cudaError_t launch_rows_i8(const RowsI8Args& a, int ftype, int sm_count, cudaStream_t stream);
 
 // Y[m*ldy + n] = (sum_k X[m*ldx + k] * W[n*ldw + k]) * xs[m] * ws[n] + bias[n], the sum exact in 32 bits (i8_matmul.cu).
 // X and W 16-byte aligned, ldx and ldw multiples of 16.
