@@ -2,19 +2,24 @@
 //
 //   m = max x,  S = sum e^(x - m),  T = sum (x - m) e^(x - m):   log p(i) = x_i - m - ln S,   H = ln S - T / S
 //
-// S and T are kept by every thread relative to its own running maximum and rescaled when that grows.  The difference to the
-// maximum is taken before anything else, so logits of any magnitude are sound and the largest has the weight 1 exactly; the
-// arithmetic is on pairs (add, mul and fma .f32x2: half an instruction a value each).  Both terms of H are at least zero, so
-// nothing cancels.
+// A warp takes 2 KB of neighbouring values at a time.  S and T are kept relative to the running maximum of what the warp has seen and
+// rescaled when that grows.  The difference to the maximum is taken before anything else, so logits of any magnitude are sound and
+// the largest has the weight 1 exactly; the arithmetic is on pairs (add, mul and fma .f32x2: half an instruction a value each).
+// Both terms of H are at least zero, so nothing cancels.
 //
-// The most likely tokens cost the pass nothing.  Values are compared as 64-bit keys (the value in the order of unsigned words,
-// below it the inverted index: the larger key is the larger value or, among equal ones, the lower index; no two are equal).
-// Every thread knows its largest value; of the keys of these, the k-th largest bounds the k-th largest of all from below, and
-// only the k threads at or above it can hold a larger one.  Their shares are read once more (k of 512 threads' values, from L2).
+// The most likely tokens cost the pass next to nothing.  Values are compared as 64-bit keys (the value in the order of unsigned
+// words, below it the inverted index: the larger key is the larger value or, among equal ones, the lower index; no two are equal).
+// The pass leaves the largest value of every block (2 KB, 512 bytes in short rows); the k best tokens lie in the k blocks that are first by largest value
+// and, among equal ones, by position: whatever lies elsewhere has a value of each of these before it.  These blocks are read once
+// more (a thread's own values, 16 bytes here and there, would cost 64 bytes of DRAM for each 16: 512 x 128256, 32 tokens, 77 us
+// against 54).
 //
 // Few rows: CTAs of a cluster share a row, so that no working memory is needed; the first of them gathers.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <cstring>
+#include <type_traits>
 
 #include "kernels.h"
 #include "q4k_common.cuh"
@@ -26,7 +31,7 @@ namespace {
 constexpr uint32_t kFull = 0xFFFFFFFFu;
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint32_t kThreads = 512, kWarps = kThreads / 32u;
+constexpr uint32_t kBlocks = 1024;  // blocks whose maxima are kept
 constexpr uint32_t kMaxGroup = 8;  // CTAs that share a row: the largest cluster that every device takes
 
 __device__ __forceinline__ float to_float(float v) { return v; }
@@ -42,6 +47,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ float max_nan(float a, float b) {  // a NaN if either is one
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+__device__ __forceinline__ float warp_max_nan(float v) {
+    float r;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
     return r;
 }
 
@@ -70,6 +81,26 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
+}
+
+// The largest of the values of U accesses, a NaN if one is; 16-bit values are compared as they are, two at a time.
+template <uint32_t U>
+__device__ __forceinline__ float largest(const uint4 (&p)[U], float) {
+    float m = __uint_as_float(p[0].x);
+#pragma unroll
+    for (uint32_t u = 0; u < U; u++)
+        m = max_nan(max_nan(max_nan(m, __uint_as_float(p[u].x)), __uint_as_float(p[u].y)), max_nan(__uint_as_float(p[u].z), __uint_as_float(p[u].w)));
+    return m;
+}
+template <uint32_t U, typename T>
+__device__ __forceinline__ float largest(const uint4 (&p)[U], T) {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    T2 m = reinterpret_cast<const T2&>(p[0].x);
+#pragma unroll
+    for (uint32_t u = 0; u < U; u++)
+        m = __hmax2_nan(__hmax2_nan(__hmax2_nan(m, reinterpret_cast<const T2&>(p[u].x)), reinterpret_cast<const T2&>(p[u].y)),
+                        __hmax2_nan(reinterpret_cast<const T2&>(p[u].z), reinterpret_cast<const T2&>(p[u].w)));
+    return max_nan(to_float(m.x), to_float(m.y));
 }
 
 // Maximum, S and T of some values, T in units of ln 2.
@@ -141,10 +172,11 @@ __device__ __forceinline__ unsigned long long merge_warp(unsigned long long a, u
 }
 
 // The best 32 of the lists of all warps, in every warp's `list`.  keys: 32 per warp; the whole CTA comes here.
+template <uint32_t WARPS>
 __device__ __forceinline__ unsigned long long merge_cta(unsigned long long list, unsigned long long (*keys)[32], uint32_t warp, uint32_t lane) {
     keys[warp][lane] = list;
 #pragma unroll
-    for (uint32_t step = kWarps / 2u; step; step >>= 1) {
+    for (uint32_t step = WARPS / 2u; step; step >>= 1) {
         __syncthreads();
         if (warp < step) keys[warp][lane] = list = merge_warp(list, keys[warp + step][lane], lane);
     }
@@ -152,9 +184,11 @@ __device__ __forceinline__ unsigned long long merge_cta(unsigned long long list,
     return keys[0][lane];
 }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const __grid_constant__ LogprobsArgs a, const uint32_t group) {
-    constexpr uint32_t E = 16 / sizeof(T), U = 16 / E, N = U * E;
+// FINE: a block is one access of a warp, else four or more.
+template <typename T, bool TOP, bool FINE, uint32_t kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(const __grid_constant__ LogprobsArgs a, const uint32_t group) {
+    constexpr uint32_t kWarps = kThreads / 32u;
+    constexpr uint32_t E = 16 / sizeof(T), U = 4;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     uint32_t rank = 0;
     if (group > 1u) {
@@ -172,17 +206,31 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const __grid_cons
     uint32_t single = a.V;
     if (rank == 0 && tid < head) single = tid;
     if (rank == group - 1u && tid >= 32u && tail + tid - 32u < a.V) single = tail + tid - 32u;
+    // lines of 32 accesses; 2^shift of them are a block, as few as the blocks' maxima have room for
+    constexpr uint32_t kStep = 32u * U;
+    const uint32_t steps = (v1 - v0 + kStep - 1u) / kStep, lines = (v1 - v0 + 31u) / 32u;
+    uint32_t shift = FINE ? 0u : 2u;
+    while ((lines >> shift) >= kBlocks) shift++;
+    const uint32_t blocks = (lines + (1u << shift) - 1u) >> shift;
+    __shared__ float s_block[TOP ? kBlocks : 1];
 
-    float m = -kInf;
-    uint64_t s2 = 0ull, t2 = 0ull;  // S and T of every other value
-    uint32_t at = 0;                // the step in which the maximum was seen first
+    // the given tokens' logits, the first of each thread: fetched now, needed at the end
+    int32_t id = -1;
+    float id_logit = 0.f;
+    if (rank == 0 && tid < a.nGiven) {
+        id = a.given[(uint64_t)row * a.nGiven + tid];
+        if (id >= 0 && (uint32_t)id < a.V) id_logit = to_float(x[id]);
+    }
+
     const uint64_t log2e2 = pair(kLog2e, kLog2e);
-    auto raise = [&](float to, uint32_t n) {
+    float m = -kInf;                // of the warp
+    uint64_t s2 = 0ull, t2 = 0ull;  // S and T of every other value
+    auto raise = [&](float to) {
         const float d = fmaxf((m - to) * kLog2e, -300.f), f = exp2_fast(d);
         const uint64_t d2 = pair(d, d), f2 = pair(f, f);
         t2 = mul2(f2, fma2(s2, d2, t2));
         s2 = mul2(f2, s2);
-        m = to, at = n;
+        m = to;
     };
     auto take = [&](float v, float w) {  // (fmaxf drops the NaN of an infinity less an infinity)
         const float2 l = halves(mul2(add2(pair(v, w), pair(-m, -m)), log2e2));
@@ -191,92 +239,111 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const __grid_cons
         s2 = add2(s2, e2);
         t2 = fma2(e2, pair(lv, lw), t2);
     };
-    for (uint32_t n = 0; v0 + tid + n * kThreads < v1; n += U) {
-        uint4 p[U];
+    auto take_access = [&](const uint4& p) {
 #pragma unroll
-        for (uint32_t u = 0; u < U; u++) {
-            const uint32_t i = v0 + tid + (n + u) * kThreads;
-            p[u] = __ldg(xv + (i < v1 ? i : v0 + tid + n * kThreads));
-        }
-        float v[N];
+        for (uint32_t j = 0; j < E; j += 2u) take(to_float(reinterpret_cast<const T*>(&p)[j]), to_float(reinterpret_cast<const T*>(&p)[j + 1u]));
+    };
+    const uint32_t block_steps = FINE ? 1u : 1u << (shift - 2u);
+    for (uint32_t b = warp; b * block_steps < steps; b += kWarps) {
+        float block = -kInf;
+        for (uint32_t step = b * block_steps; step < min(steps, (b + 1u) * block_steps); step++) {
+            const uint32_t i = v0 + step * kStep + lane;
+            uint4 p[U];
+            float mx = -kInf;
+            const bool whole = v0 + (step + 1u) * kStep <= v1;
+            if (!FINE && whole) {
 #pragma unroll
-        for (uint32_t u = 0; u < U; u++) {
-            const bool in = v0 + tid + (n + u) * kThreads < v1;
+                for (uint32_t u = 0; u < U; u++) p[u] = __ldg(xv + i + 32u * u);
+                mx = warp_max_nan(largest<U>(p, T(0.f)));
+            } else {
 #pragma unroll
-            for (uint32_t j = 0; j < E; j++) {
-                v[u * E + j] = to_float(reinterpret_cast<const T*>(&p[u])[j]);
-                if (u) v[u * E + j] = in ? v[u * E + j] : -kInf;
+                for (uint32_t u = 0; u < U; u++)
+                    if (i + 32u * u < v1) p[u] = __ldg(xv + i + 32u * u);
+#pragma unroll
+                for (uint32_t u = 0; u < U; u++) {
+                    const uint4 one[1] = {p[u]};
+                    const float line = warp_max_nan(i + 32u * u < v1 ? largest<1>(one, T(0.f)) : -kInf);
+                    mx = max_nan(mx, line);
+                    if (TOP && FINE && lane == 0 && step * U + u < lines && BPQ4K_CHECK(lines <= kBlocks, a.status)) s_block[step * U + u] = line;
+                }
             }
+            if (!(mx <= m)) raise(max_nan(mx, m));
+            block = fmaxf(block, mx);
+#pragma unroll
+            for (uint32_t u = 0; u < U; u++)
+                if (whole || i + 32u * u < v1) take_access(p[u]);
         }
-        float mx = v[0];
-#pragma unroll
-        for (uint32_t j = 1; j < N; j++) mx = max_nan(mx, v[j]);
-        if (!(mx <= m)) raise(max_nan(mx, m), n);
-#pragma unroll
-        for (uint32_t j = 0; j < N; j += 2u) take(v[j], v[j + 1u]);
+        if (TOP && !FINE && lane == 0 && BPQ4K_CHECK(b < blocks, a.status)) s_block[b] = block;
     }
-    const float own = m;  // of the accesses alone
-    const uint32_t own_at = at;
-    if (single < a.V) {
-        const float v = to_float(x[single]);
-        if (!(v <= m)) raise(max_nan(v, m), 0u);
+    if (warp < 2u) {
+        const float v = single < a.V ? to_float(x[single]) : -kInf, mx = warp_max_nan(v);
+        if (!(mx <= m)) raise(max_nan(mx, m));
         take(v, -kInf);
     }
     Stats st{m, halves(s2).x + halves(s2).y, halves(t2).x + halves(t2).y};
 
     __shared__ unsigned long long s_keys[kWarps][32];
     __shared__ Stats s_stats[kWarps];
+    __shared__ unsigned long long s_found[TOP ? kThreads : 1];
+    __shared__ uint32_t s_count;
     __shared__ unsigned long long c_keys[TOP ? kMaxGroup : 1][32];
     __shared__ Stats c_stats[kMaxGroup];
     st.add_lanes();
     if (lane == 0) s_stats[warp] = st;
     unsigned long long list = 0ull;
     if constexpr (TOP) {
-        unsigned long long key = 0ull;
-        if (v0 + tid < v1) {  // where in its step the maximum is
-            uint32_t idx = 0xFFFFFFFFu;
-#pragma unroll
-            for (uint32_t u = U; u-- > 0u;) {
-                const uint32_t i = v0 + tid + (own_at + u) * kThreads;
-                if (i >= v1) continue;
-                const uint4 p = __ldg(xv + i);
-#pragma unroll
-                for (uint32_t j = E; j-- > 0u;)
-                    if (to_float(reinterpret_cast<const T*>(&p)[j]) == own) idx = head + i * E + j;
-            }
-            key = make_key(own, idx);
-        }
-        const unsigned long long best = merge_cta(sort_warp(key, lane), s_keys, warp, lane);  // lane i: the i-th of the threads' best keys
-        const unsigned long long bound = __shfl_sync(kFull, best, a.nTop - 1u);
-        unsigned long long least = bound ? bound - 1ull : 0ull;  // what a key has to exceed
-        auto offer = [&](unsigned long long k) {  // a key of every lane, 0: none
-            uint32_t who = __ballot_sync(kFull, k > least);
-            while (who) {
-                const unsigned long long c = __shfl_sync(kFull, k, __ffs(who) - 1u);
-                who &= who - 1u;
-                if (c <= least) continue;
-                const uint32_t pos = __popc(__ballot_sync(kFull, list > c));
-                const unsigned long long up = __shfl_up_sync(kFull, list, 1);
-                if (lane >= pos) list = lane == pos ? c : up;
-                const unsigned long long last = __shfl_sync(kFull, list, a.nTop - 1u);
-                least = last > least ? last : least;
-            }
-        };
-        for (uint32_t w = warp; w < a.nTop; w += kWarps) {
-            const unsigned long long k = __shfl_sync(kFull, best, w);
-            if (k == 0ull) break;
-            const uint32_t t = ((key_index(k) - head) / E - v0) % kThreads;
-            for (uint32_t i0 = v0 + t; i0 < v1; i0 += 32u * kThreads) {
-                const uint32_t i = i0 + lane * kThreads;
-                uint4 p = make_uint4(0u, 0u, 0u, 0u);
-                if (BPQ4K_CHECK(t < kThreads, a.status) && i < v1) p = __ldg(xv + i);
-#pragma unroll
-                for (uint32_t j = 0; j < E; j++) offer(i < v1 ? make_key(to_float(reinterpret_cast<const T*>(&p)[j]), head + i * E + j) : 0ull);
-            }
-        }
-        if (warp < 2u) offer(single < a.V ? make_key(to_float(x[single]), single) : 0ull);
         __syncthreads();
-        list = merge_cta(list, s_keys, warp, lane);
+        // the k first blocks: lane i has the i-th
+        unsigned long long best = 0ull;
+        for (uint32_t b = warp * 32u; b < blocks; b += kThreads) {
+            const unsigned long long k = sort_warp(b + lane < blocks ? make_key(s_block[b + lane], b + lane) : 0ull, lane);
+            best = b < kThreads ? k : merge_warp(best, k, lane);
+        }
+        best = merge_cta<kWarps>(best, s_keys, warp, lane);
+        const unsigned long long bound = __shfl_sync(kFull, best, a.nTop - 1u);
+        // what a key has to exceed: the k-th block has a value like its largest, at its end if nowhere else
+        unsigned long long least = 0ull;
+        if (bound) least = make_key(key_value(bound), head + min(v1, v0 + ((key_index(bound) + 1u) << shift) * 32u) * E - 1u) - 1ull;
+        // Keys above `least` are collected, a few more than k as a rule.  Should they not fit, the k-th of those that did is a better
+        // bound, and the blocks are read again.
+        for (;;) {
+            if (tid == 0) s_count = 0u;
+            s_found[tid] = 0ull;
+            __syncthreads();
+            auto offer = [&](unsigned long long k) {
+                if (k <= least) return;
+                const uint32_t at = atomicAdd(&s_count, 1u);
+                if (at < kThreads) s_found[at] = k;
+            };
+            for (uint32_t w = warp; w < a.nTop; w += kWarps) {
+                const unsigned long long k = __shfl_sync(kFull, best, w);
+                if (k == 0ull) break;
+                const uint32_t b = key_index(k);
+                constexpr uint32_t R = FINE ? 1u : 4u;
+                for (uint32_t line = b << shift; line < min(lines, (b + 1u) << shift); line += R) {
+                    const uint32_t i = v0 + line * 32u + lane;
+                    uint4 p[R];
+#pragma unroll
+                    for (uint32_t u = 0; u < R; u++)
+                        if (BPQ4K_CHECK(line < lines, a.status) && i + 32u * u < v1) p[u] = __ldg(xv + i + 32u * u);
+#pragma unroll
+                    for (uint32_t u = 0; u < R; u++)
+#pragma unroll
+                        for (uint32_t j = 0; j < E; j++)
+                            if (i + 32u * u < v1) offer(make_key(to_float(reinterpret_cast<const T*>(&p[u])[j]), head + (i + 32u * u) * E + j));
+                }
+            }
+            if (single < a.V) offer(make_key(to_float(x[single]), single));
+            __syncthreads();
+            const uint32_t found = s_count;
+            list = s_found[tid];
+            if (found > 32u || warp == 0) list = sort_warp(list, lane);
+            if (found > 32u) list = merge_cta<kWarps>(list, s_keys, warp, lane);
+            if (found <= kThreads) break;
+            least = __shfl_sync(kFull, list, a.nTop - 1u) - 1ull;
+            __syncthreads();
+        }
+        __syncthreads();
     } else {
         __syncthreads();
     }
@@ -303,9 +370,11 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const __grid_cons
     const float ln_s = logf(st.s), nan = __uint_as_float(0x7FC00000u);
     auto logp = [&](float v) { return bad ? nan : none || v == -kInf ? -kInf : (float)((double)v - (double)st.m - (double)ln_s); };
     if (a.entropy && tid == 0) a.entropy[row] = bad ? nan : none ? 0.f : ln_s - 0.69314718056f * (st.t / st.s);
-    for (uint32_t g = tid; g < a.nGiven; g += kThreads) {
-        const int32_t id = a.given[(uint64_t)row * a.nGiven + g];
-        a.given_lp[(uint64_t)row * a.nGiven + g] = id < 0 || (uint32_t)id >= a.V ? nan : logp(to_float(x[id]));
+    auto is_token = [&](int32_t i) { return i >= 0 && (uint32_t)i < a.V; };
+    if (tid < a.nGiven) a.given_lp[(uint64_t)row * a.nGiven + tid] = is_token(id) ? logp(id_logit) : nan;
+    for (uint32_t g = tid + kThreads; g < a.nGiven; g += kThreads) {
+        id = a.given[(uint64_t)row * a.nGiven + g];
+        a.given_lp[(uint64_t)row * a.nGiven + g] = is_token(id) ? logp(to_float(x[id])) : nan;
     }
     if (TOP && tid < a.nTop) {
         a.top_ids[(uint64_t)row * a.nTop + tid] = bad ? -1 : (int32_t)key_index(list);
@@ -313,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const __grid_cons
     }
 }
 
-template <typename T, bool TOP>
+template <typename T, bool TOP, bool FINE, uint32_t kThreads>
 cudaError_t launch_rows(const LogprobsArgs& a, uint32_t group, cudaStream_t stream) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(a.M * group);
@@ -324,15 +393,20 @@ cudaError_t launch_rows(const LogprobsArgs& a, uint32_t group, cudaStream_t stre
     attr[0].val.clusterDim.x = group, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = group > 1u ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, TOP>, a, group);
+    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, TOP, FINE, kThreads>, a, group);
 }
 
 template <typename T>
 cudaError_t launch_type(const LogprobsArgs& a, int sm_count, cudaStream_t stream) {
-    // CTAs that share a row: while there are SMs without one, and a thread has a step's work
+    // CTAs that share a row: while they are fewer than the machine holds at once, and a thread has 16 values
     uint32_t group = 1;
-    while (group < kMaxGroup && a.M * group * 2u <= 2u * (uint32_t)sm_count && a.V >= group * 2u * kThreads * 8u) group *= 2u;
-    return a.nTop ? launch_rows<T, true>(a, group, stream) : launch_rows<T, false>(a, group, stream);
+    while (group < kMaxGroup && (uint64_t)a.M * group * 2u <= 4ull * sm_count && a.V >= group * 2u * 4096u) group *= 2u;
+    if (!a.nTop) return launch_rows<T, false, false, 256>(a, group, stream);
+    // fine blocks where there are too few of the others for the most that can be asked of a CTA's part of a row
+    if (a.V / group >= kLogprobsMaxTop * (2048u / (uint32_t)sizeof(T))) return launch_rows<T, true, false, 256>(a, group, stream);
+    // (512 x 4000 float: 128 threads 7.7 us, 256 8.7; 8 x 128256, eight CTAs a row: 11.0 and 9.0)
+    if (a.V / group > 4096u) return launch_rows<T, true, true, 256>(a, group, stream);
+    return launch_rows<T, true, true, 128>(a, group, stream);
 }
 
 }  // namespace
