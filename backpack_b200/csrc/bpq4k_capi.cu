@@ -1105,9 +1105,9 @@ int bpq4k_matmul_i8(bpq4k_handle_t h, int ftype, const int8_t* X, const float* x
     DeviceGuard g(h->device);
     MatmulI8Args a{};
     a.X = X, a.xs = x_scales, a.W = W, a.ws = w_scales, a.bias = bias, a.Y = Y;
-    a.M = M, a.N = N, a.K = K, a.ldx = ldx, a.ldw = ldw, a.ldy = ldy;
+    a.M = M, a.N = N, a.K = K, a.ldx = ldx, a.ldw = ldw, a.ldy = ldy, a.status = h->dev_status;
     int launches = 0;
-    const cudaError_t e = launch_matmul_i8(a, ftype, h->dev_status, h->sm_count, static_cast<cudaStream_t>(stream), &launches);
+    const cudaError_t e = launch_matmul_i8(a, ftype, h->sm_count, static_cast<cudaStream_t>(stream), &launches);
     h->launches += (uint64_t)launches;
     if (e != cudaSuccess) return cuda_fail(h, e, "8-bit matmul launch");
     return BPQ4K_OK;

@@ -36,6 +36,97 @@ __device__ __forceinline__ __nv_bfloat16 to_elem<__nv_bfloat16>(float v) { retur
 // The same three roundings in every kernel: the sum to a float, its product with xs, and that times ws plus the bias.
 __device__ __forceinline__ float finish(int s, float xs, float ws, float bias) { return fmaf(__fmul_rn((float)s, xs), ws, bias); }
 
+// ---- few activation rows: weights straight into registers ---------------------------------------------------------------
+
+
+// 16 codes from byte k of a row on: zeros behind the row, and (`clean`) in place of the bytes behind code K.
+__device__ __forceinline__ int4 codes16(const int8_t* row, uint32_t k, uint32_t K, bool clean) {
+    if (k >= K) return make_int4(0, 0, 0, 0);
+    int4 v = __ldg(reinterpret_cast<const int4*>(row + k));
+    if (clean && k + 16u > K) {
+        const uint32_t n = K - k;  // 1..15 codes
+        auto keep = [n](int w, uint32_t first) { return n >= first + 4u ? w : n <= first ? 0 : w & (int)((1u << (8u * (n - first))) - 1u); };
+        v.x = keep(v.x, 0), v.y = keep(v.y, 4), v.z = keep(v.z, 8), v.w = keep(v.w, 12);
+    }
+    return v;
+}
+__device__ __forceinline__ void mma_i8(int (&c)[4], int a0, int a1, int a2, int a3, int b0, int b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+constexpr uint32_t kStreamRows = 8;  // activation rows at most: the mma's columns
+
+// A warp takes 16 weight rows and a share of K; 2^wk_log warps of the CTA share the rows.  Lane (g, t) = (lane / 4, lane % 4) loads
+// the 16 bytes 64 p + 16 t of rows g and g + 8 and of activation row g: which codes of K meet in one mma does not matter as long as
+// both operands agree, so a lane's 16 bytes are the fragments of two mmas as they are.  No shared memory, tensor memory or barrier
+// stands between the launch and the first load: 1 x 1024 x 4096 3.7 us, by the kernel below 6.0; 1 x 4096 x 4096 5.7 and 7.6;
+// 4 x 6144 x 4096 8.1 and 9.4.  Its loads are 64 bytes of 16 rows at a time, which DRAM likes less than whole boxes: 1 x 14336 x
+// 4096 12.8 us both, 8 x 28672 x 8192 50 and 44.
+template <typename T, uint32_t kStreamWarps>
+__global__ void __launch_bounds__(kStreamWarps * 32, 1024 / (kStreamWarps * 32)) matmul_i8_stream_kernel(const __grid_constant__ MatmulI8Args a, const uint32_t wk_log) {
+    constexpr uint32_t kStreamThreads = kStreamWarps * 32, kPieces = 4;  // 64-byte pieces of a row in flight
+    __shared__ int parts[kStreamWarps][16][8];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+    const uint32_t tiles = kStreamWarps >> wk_log, n0 = (blockIdx.x * tiles + (warp >> wk_log)) * 16u, share = warp & ((1u << wk_log) - 1u);
+    const uint32_t pieces = (a.K + 63u) / 64u;
+    const uint32_t p0 = (uint32_t)((uint64_t)pieces * share >> wk_log), p1 = (uint32_t)((uint64_t)pieces * (share + 1u) >> wk_log);
+    const int8_t* w0 = a.W + (uint64_t)min(n0 + g, a.N - 1u) * a.ldw;
+    const int8_t* w1 = a.W + (uint64_t)min(n0 + g + 8u, a.N - 1u) * a.ldw;
+    const int8_t* x = a.X + (uint64_t)min(g, a.M - 1u) * a.ldx;
+    int c[4] = {};
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // all that is read comes from earlier kernels
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // the scales of this thread's first output: needed at the end, fetched now
+    const uint32_t rows = tiles * 16u, m_first = threadIdx.x / rows, n_first = blockIdx.x * rows + threadIdx.x % rows;
+    const bool first = m_first < a.M && n_first < a.N;
+    const float xs_first = first ? __ldg(a.xs + m_first) : 0.f, ws_first = first ? __ldg(a.ws + n_first) : 0.f;
+    const float bias_first = first && a.bias ? __ldg(a.bias + n_first) : 0.f;
+    for (uint32_t p = p0; p < p1; p += kPieces) {
+        int4 u[kPieces], v[kPieces];
+#pragma unroll
+        for (uint32_t i = 0; i < kPieces; i++) {
+            const uint32_t k = p + i < p1 ? (p + i) * 64u + t * 16u : a.K;
+            u[i] = codes16(w0, k, a.K, false);
+            v[i] = codes16(w1, k, a.K, false);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kPieces; i++) {
+            const uint32_t k = p + i < p1 ? (p + i) * 64u + t * 16u : a.K;
+            const int4 b = codes16(x, k, a.K, true);
+            mma_i8(c, u[i].x, v[i].x, u[i].y, v[i].y, b.x, b.y);
+            mma_i8(c, u[i].z, v[i].z, u[i].w, v[i].w, b.z, b.w);
+        }
+    }
+    *reinterpret_cast<int2*>(&parts[warp][g][2u * t]) = make_int2(c[0], c[1]);
+    *reinterpret_cast<int2*>(&parts[warp][g + 8u][2u * t]) = make_int2(c[2], c[3]);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < rows * a.M; i += kStreamThreads) {
+        const uint32_t m = i / rows, r = i - m * rows, n = blockIdx.x * rows + r;
+        if (n >= a.N || !BPQ4K_CHECK(m < a.M && m < kStreamRows, a.status)) continue;
+        int sum = 0;
+        for (uint32_t s = 0; s < 1u << wk_log; s++) sum += parts[((r >> 4) << wk_log) + s][r & 15u][m];
+        static_cast<T*>(a.Y)[(uint64_t)m * a.ldy + n] = to_elem<T>(
+            i < kStreamThreads ? finish(sum, xs_first, ws_first, bias_first) : finish(sum, __ldg(a.xs + m), __ldg(a.ws + n), a.bias ? __ldg(a.bias + n) : 0.f));
+    }
+}
+
+template <typename T, uint32_t kStreamWarps>
+cudaError_t launch_stream(const MatmulI8Args& m, uint32_t wk_log, cudaStream_t stream) {
+    const uint32_t rows = (kStreamWarps >> wk_log) * 16u;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((m.N + rows - 1u) / rows);
+    cfg.blockDim = dim3(kStreamWarps * 32);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, matmul_i8_stream_kernel<T, kStreamWarps>, m, wk_log);
+}
+
 // ---- tensor cores -------------------------------------------------------------------------------------------------------
 
 constexpr uint32_t kWaitLimit = 1u << 21;
@@ -43,6 +134,7 @@ constexpr uint32_t kSuspendNs = 1000;
 constexpr uint32_t kStep = 128;                       // codes of a row per ring stage: the swizzle's row
 constexpr uint32_t kEpilogueWarps = 8, kThreads = (4 + kEpilogueWarps) * 32;
 constexpr uint32_t kMaxStages = 12;
+constexpr uint32_t kMaxSplits = 8;                    // CTAs that share a tile: the largest cluster that every device takes
 constexpr uint32_t kMaxTile = 256;                    // activation rows of a tile
 
 struct TcArgs {
@@ -150,6 +242,12 @@ __device__ __forceinline__ void umma_commit(uint32_t bar) {
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* v) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
@@ -202,6 +300,10 @@ __global__ void __launch_bounds__(kThreads, 2) matmul_i8_kernel(const __grid_con
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 0 && lane == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&a.tmap_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&a.tmap_x) : "memory");
     }
     if (warp == 2) {
         if constexpr (CG == 1) {
@@ -304,30 +406,28 @@ __global__ void __launch_bounds__(kThreads, 2) matmul_i8_kernel(const __grid_con
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(peer_addr(acc_empty(buf), CG == 2 ? 0u : rank));
             } else {
-                // every CTA of the cluster has a part of each sum: CTA q adds up and stores the q-th share of the columns
-                const uint32_t share = a.tile / a.splits;
-                for (uint32_t c = side * 16u; c < cols && ok; c += 32u) {
-                    uint32_t v[16];
-                    tmem_ld16(acc + c, v);
+                // every CTA of the cluster has a part of each sum: CTA q adds up and stores the columns that are q modulo the CTAs
+                const uint32_t mask = a.splits - 1u, log = 31u - __clz(a.splits), share = a.tile >> log;
+                const uint32_t slot = exchange + (rank * share * 128u + r) * 4u;
+                for (uint32_t c = side * 8u; c < cols && ok; c += 16u) {
+                    uint32_t v[8];
+                    tmem_ld8(acc + c, v);
 #pragma unroll
-                    for (uint32_t j = 0; j < 16; j++) {
-                        const uint32_t q = (c + j) / share;
+                    for (uint32_t j = 0; j < 8; j++)
                         if (c + j < cols)
-                            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_addr(exchange, q) + ((rank * share + (c + j) - q * share) * 128u + r) * 4u),
-                                         "r"(v[j])
-                                         : "memory");
-                    }
+                            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_addr(slot + ((c + j) >> log) * 512u, j & mask)), "r"(v[j]) : "memory");
                 }
                 asm volatile("fence.acq_rel.cluster;" ::: "memory");
                 __syncwarp();
-                if (lane == 0)
-                    for (uint32_t q = 0; q < a.splits; q++) mbar_arrive_cluster(peer_addr(parts_bar, q));
+                if (lane < a.splits) mbar_arrive_cluster(peer_addr(parts_bar, lane));
                 const bool all = wait_bar(parts_bar, 0u, abort_flag, a.status);
-                const int* parts = reinterpret_cast<const int*>(base_ptr + off_bar + kBarBytes);
-                for (uint32_t c = side; c < share && rank * share + c < cols && all && live; c += 2u) {
+                const int* parts = reinterpret_cast<const int*>(base_ptr + off_bar + kBarBytes) + r;
+                for (uint32_t c = side; rank + (c << log) < cols && all && live; c += 2u) {
                     int sum = 0;
-                    for (uint32_t p = 0; p < a.splits; p++) sum += parts[(p * share + c) * 128u + r];
-                    const uint32_t m = rank * share + c;
+#pragma unroll
+                    for (uint32_t p = 0; p < kMaxSplits; p++)
+                        if (p < a.splits) sum += parts[(p * share + c) * 128u];
+                    const uint32_t m = rank + (c << log);
                     Y[(uint64_t)(m0 + m) * a.ldy + n] = to_elem<T>(finish(sum, xscale[m], wscale, bias));
                 }
             }
@@ -368,25 +468,44 @@ bool encode_rows(CUtensorMap* map, const int8_t* codes, uint32_t rows, uint32_t 
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// How a product is cut: activation rows of a tile, tiles, CTAs that share a tile's K range.
+struct Cut {
+    uint32_t tile, m_tiles, splits;
+    uint64_t tiles;
+    double us;  // estimate of what differs between cuts
+};
+// An SM takes in about 92 GB/s (32 SMs streaming weights; 128 x 256 tiles of a pair), so a step costs what both operands' bytes of a
+// stage do; a shared tile costs an exchange.  (128 x 4096 x 14336: a pair 33 us, four CTAs to a tile 17.7.)
+template <int CG>
+Cut cut_of(const MatmulI8Args& m, int sm_count) {
+    Cut c{};
+    const uint32_t most = CG == 1 ? kMaxTile / 2u : kMaxTile, unit = CG * 16u;  // (the mma's step of N)
+    c.m_tiles = (m.M + most - 1u) / most;
+    c.tile = ((m.M + c.m_tiles - 1u) / c.m_tiles + unit - 1u) / unit * unit;
+    c.m_tiles = (m.M + c.tile - 1u) / c.tile;
+    c.tiles = (uint64_t)((m.N + CG * 128u - 1u) / (CG * 128u)) * c.m_tiles;
+    c.splits = 1;
+    const uint32_t chunks = (m.K + kStep - 1u) / kStep;
+    if (CG == 1)
+        while (c.splits < kMaxSplits && c.tiles * c.splits * 2u <= (uint32_t)sm_count && chunks >= c.splits * 8u) c.splits *= 2u;
+    const uint64_t groups = (uint32_t)sm_count / (CG * c.splits), rounds = (c.tiles + groups - 1u) / groups;
+    c.us = (double)rounds * ((chunks + c.splits - 1u) / c.splits) * stage_bytes(c.tile, CG) / 92e3 + (c.splits > 1u ? 1.0 + 0.012 * c.tile : 0.0);
+    return c;
+}
+
 template <int CG, typename T>
-cudaError_t launch_tc(const MatmulI8Args& m, int* status_dev, int sm_count, cudaStream_t stream) {
+cudaError_t launch_tc(const MatmulI8Args& m, const Cut& cut, int sm_count, cudaStream_t stream) {
     TcArgs a{};
-    a.xs = m.xs, a.ws = m.ws, a.bias = m.bias, a.Y = m.Y, a.M = m.M, a.N = m.N, a.ldy = m.ldy, a.status = status_dev;
-    const uint32_t unit = CG * 16u;  // the mma's step of N
-    a.m_tiles = (m.M + kMaxTile - 1u) / kMaxTile;
-    a.tile = ((m.M + a.m_tiles - 1u) / a.m_tiles + unit - 1u) / unit * unit;
-    a.m_tiles = (m.M + a.tile - 1u) / a.tile;
+    a.xs = m.xs, a.ws = m.ws, a.bias = m.bias, a.Y = m.Y, a.M = m.M, a.N = m.N, a.ldy = m.ldy, a.status = m.status;
     a.chunks = (m.K + kStep - 1u) / kStep;
-    const uint64_t tiles = (uint64_t)((m.N + CG * 128u - 1u) / (CG * 128u)) * a.m_tiles;
-    if (tiles > 0x7FFFFFFFull) return cudaErrorInvalidValue;
-    a.tiles = (uint32_t)tiles;
-    a.splits = 1;
-    if (CG == 1)  // few tiles: up to eight CTAs share the K range of one
-        while (a.splits < 8u && a.tile <= 64u && a.tiles * a.splits * 2u <= 2u * (uint32_t)sm_count && a.chunks >= a.splits * 4u) a.splits *= 2u;
+    if (cut.tiles > 0x7FFFFFFFull) return cudaErrorInvalidValue;
+    a.tile = cut.tile, a.m_tiles = cut.m_tiles, a.tiles = (uint32_t)cut.tiles, a.splits = cut.splits;
+    // (a shorter ring is faster where little else than weights is read: 1 x 128256 x 4096 79 us with 150 KB, 85 with 226)
+    const uint32_t budget = (a.tile <= 48u ? 150u : 226u) * 1024u;
     const uint32_t group = CG == 2 ? 2u : a.splits;
-    const uint32_t budget = a.splits > 1u ? 112u * 1024u : 226u * 1024u;
     a.stages = (budget - smem_bytes(0, a.tile, CG, a.splits)) / stage_bytes(a.tile, CG);
     if (a.stages > kMaxStages) a.stages = kMaxStages;
+    if (a.stages < 2u) return cudaErrorInvalidValue;
     a.tmem_cols = 32;
     while (a.tmem_cols < (a.splits > 1u ? 1u : 2u) * a.tile) a.tmem_cols *= 2u;
     uint32_t groups = (uint32_t)sm_count / group;
@@ -411,19 +530,27 @@ cudaError_t launch_tc(const MatmulI8Args& m, int* status_dev, int sm_count, cuda
 }
 
 template <typename T>
-cudaError_t launch_type(const MatmulI8Args& a, int* status_dev, int sm_count, cudaStream_t stream) {
-    return a.M <= 64u ? launch_tc<1, T>(a, status_dev, sm_count, stream) : launch_tc<2, T>(a, status_dev, sm_count, stream);
+cudaError_t launch_type(const MatmulI8Args& a, int sm_count, cudaStream_t stream) {
+    if (a.M <= kStreamRows && (uint64_t)a.N * a.K <= 32u << 20) {
+        // warps that share a row tile: as many as keep all warps on the machine at once (32 an SM) and leave each a fetch of its own
+        const uint64_t tiles = (a.N + 15u) / 16u, fetches = (a.K + 255u) / 256u;
+        uint32_t wk_log = 0;
+        while (wk_log < 4u && tiles << (wk_log + 1u) <= 32u * (uint64_t)sm_count && fetches >> (wk_log + 1u)) wk_log++;
+        return wk_log == 4u ? launch_stream<T, 16>(a, wk_log, stream) : launch_stream<T, 8>(a, wk_log, stream);
+    }
+    const Cut one = cut_of<1>(a, sm_count), pair = cut_of<2>(a, sm_count);
+    return one.us <= pair.us ? launch_tc<1, T>(a, one, sm_count, stream) : launch_tc<2, T>(a, pair, sm_count, stream);
 }
 
 }  // namespace
 
-cudaError_t launch_matmul_i8(const MatmulI8Args& a, int ftype, int* status_dev, int sm_count, cudaStream_t stream, int* launches) {
+cudaError_t launch_matmul_i8(const MatmulI8Args& a, int ftype, int sm_count, cudaStream_t stream, int* launches) {
     if (a.M == 0 || a.N == 0) return cudaSuccess;
     ++*launches;
     switch (ftype) {
-        case 0: return launch_type<float>(a, status_dev, sm_count, stream);
-        case 1: return launch_type<__half>(a, status_dev, sm_count, stream);
-        case 30: return launch_type<__nv_bfloat16>(a, status_dev, sm_count, stream);
+        case 0: return launch_type<float>(a, sm_count, stream);
+        case 1: return launch_type<__half>(a, sm_count, stream);
+        case 30: return launch_type<__nv_bfloat16>(a, sm_count, stream);
         default: return cudaErrorInvalidValue;
     }
 }

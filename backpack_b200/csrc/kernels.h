@@ -190,8 +190,9 @@ struct MatmulI8Args {
     const float* bias;  // may be null
     void* Y;
     uint32_t M, N, K, ldx, ldw, ldy;
+    int* status;
 };
-cudaError_t launch_matmul_i8(const MatmulI8Args& a, int ftype, int* status_dev, int sm_count, cudaStream_t stream, int* launches);
+cudaError_t launch_matmul_i8(const MatmulI8Args& a, int ftype, int sm_count, cudaStream_t stream, int* launches);
 
 // Log probabilities of given tokens, entropy, most likely tokens of every row of logits (bpq4k_logprobs.cu).
 constexpr uint32_t kLogprobsMaxTop = 32;
