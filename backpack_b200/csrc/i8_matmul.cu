@@ -146,6 +146,7 @@ struct TcArgs {
     uint32_t M, N, ldy;
     uint32_t tile, m_tiles, tiles, chunks;  // activation rows of a tile, tiles along M, tiles in all, steps along K
     uint32_t splits;                        // CTAs that share a tile's K range (one CTA form)
+    uint32_t in_ring;                       // where they exchange their sums: 1 the ring (once it is free), 0 behind the barriers
     uint32_t stages, tmem_cols;
     int* status;
 };
@@ -260,9 +261,9 @@ __device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, %0;"
 // Shared memory behind the ring: activation scales of two tiles, barriers, flags; the exchange of a shared tile.
 constexpr uint32_t kScaleBytes = 2u * kMaxTile * 4u, kBarBytes = 512u;
 constexpr uint32_t stage_bytes(uint32_t tile, uint32_t cg) { return 128u * kStep + tile / cg * kStep; }
-constexpr uint32_t exchange_bytes(uint32_t tile, uint32_t splits) { return splits > 1u ? tile * 128u * 4u : 0u; }
-constexpr uint32_t smem_bytes(uint32_t stages, uint32_t tile, uint32_t cg, uint32_t splits) {
-    return 1024u + stages * stage_bytes(tile, cg) + kScaleBytes + kBarBytes + exchange_bytes(tile, splits);
+constexpr uint32_t exchange_bytes(uint32_t tile) { return tile * 128u * 4u; }
+constexpr uint32_t smem_bytes(uint32_t stages, uint32_t tile, uint32_t cg, bool exchange) {
+    return 1024u + stages * stage_bytes(tile, cg) + kScaleBytes + kBarBytes + (exchange ? exchange_bytes(tile) : 0u);
 }
 
 template <int CG, typename T>
@@ -272,30 +273,31 @@ __global__ void __launch_bounds__(kThreads, 2) matmul_i8_kernel(const __grid_con
     uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
     const uint32_t sbytes = stage_bytes(a.tile, CG), off_scale = a.stages * sbytes, off_bar = off_scale + kScaleBytes;
     float* scale = reinterpret_cast<float*>(base_ptr + off_scale);
-    const uint32_t bar0 = base + off_bar, exchange = bar0 + kBarBytes;
+    const uint32_t bar0 = base + off_bar, off_exchange = a.in_ring ? 0u : off_bar + kBarBytes;
     auto full = [&](uint32_t s) { return bar0 + s * 8u; };
     auto empty = [&](uint32_t s) { return bar0 + (kMaxStages + s) * 8u; };
     auto acc_full = [&](uint32_t b) { return bar0 + (2u * kMaxStages + b) * 8u; };
     auto acc_empty = [&](uint32_t b) { return bar0 + (2u * kMaxStages + 2u + b) * 8u; };
-    const uint32_t parts_bar = bar0 + (2u * kMaxStages + 4u) * 8u, done_bar = parts_bar + 8u;
+    const uint32_t parts_bar = bar0 + (2u * kMaxStages + 4u) * 8u, done_bar = parts_bar + 8u, ready_bar = parts_bar + 24u;
     static_assert((2u * kMaxStages + 8u) * 8u <= kBarBytes, "barrier area");
     volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + off_bar + (2u * kMaxStages + 6u) * 8u);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + off_bar + (2u * kMaxStages + 6u) * 8u + 4u);
 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     uint32_t rank = 0;
-    if (CG == 2 || a.splits > 1u) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     const uint32_t group = CG == 2 ? 2u : a.splits;            // CTAs of a cluster
+    if (group > 1u) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     const uint32_t first_tile = blockIdx.x / group, step_tile = gridDim.x / group;
     const uint32_t half = CG == 2 ? rank : 0u;                 // which half of the pair's operands
-    const bool leader = CG == 1 || rank == 0u;
-    const uint32_t c0 = CG == 2 ? 0u : (uint32_t)((uint64_t)a.chunks * rank / a.splits);
-    const uint32_t c1 = CG == 2 ? a.chunks : (uint32_t)((uint64_t)a.chunks * (rank + 1u) / a.splits);
+    const uint32_t part = CG == 2 ? 0u : rank;                 // which share of K
+    const bool leader = half == 0u;
+    const uint32_t c0 = (uint32_t)((uint64_t)a.chunks * part / a.splits), c1 = (uint32_t)((uint64_t)a.chunks * (part + 1u) / a.splits);
 
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < a.stages; s++) mbar_init(full(s), 1), mbar_init(empty(s), 1);
         for (uint32_t b = 0; b < 2; b++) mbar_init(acc_full(b), 1), mbar_init(acc_empty(b), CG * kEpilogueWarps);
-        mbar_init(parts_bar, group * kEpilogueWarps);
+        mbar_init(parts_bar, a.splits * kEpilogueWarps);
+        mbar_init(ready_bar, a.splits);
         mbar_init(done_bar, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -407,9 +409,14 @@ __global__ void __launch_bounds__(kThreads, 2) matmul_i8_kernel(const __grid_con
                 if (lane == 0) mbar_arrive_cluster(peer_addr(acc_empty(buf), CG == 2 ? 0u : rank));
             } else {
                 // every CTA of the cluster has a part of each sum: CTA q adds up and stores the columns that are q modulo the CTAs
-                const uint32_t mask = a.splits - 1u, log = 31u - __clz(a.splits), share = a.tile >> log;
-                const uint32_t slot = exchange + (rank * share * 128u + r) * 4u;
-                for (uint32_t c = side * 8u; c < cols && ok; c += 16u) {
+                const uint32_t mask = a.splits - 1u, log = 31u - __clz(a.splits), cols_each = a.tile >> log;
+                const uint32_t slot = base + off_exchange + (part * cols_each * 128u + r) * 4u;
+                bool ready = ok;
+                if (a.in_ring) {  // this CTA's mmas are done with its ring; the others'?
+                    if (e < a.splits) mbar_arrive_cluster(peer_addr(ready_bar, e));
+                    ready = wait_bar(ready_bar, 0u, abort_flag, a.status) && ok;
+                }
+                for (uint32_t c = side * 8u; c < cols && ready; c += 16u) {
                     uint32_t v[8];
                     tmem_ld8(acc + c, v);
 #pragma unroll
@@ -421,13 +428,13 @@ __global__ void __launch_bounds__(kThreads, 2) matmul_i8_kernel(const __grid_con
                 __syncwarp();
                 if (lane < a.splits) mbar_arrive_cluster(peer_addr(parts_bar, lane));
                 const bool all = wait_bar(parts_bar, 0u, abort_flag, a.status);
-                const int* parts = reinterpret_cast<const int*>(base_ptr + off_bar + kBarBytes) + r;
-                for (uint32_t c = side; rank + (c << log) < cols && all && live; c += 2u) {
+                const int* parts = reinterpret_cast<const int*>(base_ptr + off_exchange) + r;
+                for (uint32_t c = side; part + (c << log) < cols && all && live; c += 2u) {
                     int sum = 0;
 #pragma unroll
                     for (uint32_t p = 0; p < kMaxSplits; p++)
-                        if (p < a.splits) sum += parts[(p * share + c) * 128u];
-                    const uint32_t m = rank + (c << log);
+                        if (p < a.splits) sum += parts[(p * cols_each + c) * 128u];
+                    const uint32_t m = part + (c << log);
                     Y[(uint64_t)(m0 + m) * a.ldy + n] = to_elem<T>(finish(sum, xscale[m], wscale, bias));
                 }
             }
@@ -476,6 +483,10 @@ struct Cut {
 };
 // An SM takes in about 92 GB/s (32 SMs streaming weights; 128 x 256 tiles of a pair), so a step costs what both operands' bytes of a
 // stage do; a shared tile costs an exchange.  (128 x 4096 x 14336: a pair 33 us, four CTAs to a tile 17.7.)
+constexpr uint32_t kSmem = 226u * 1024u;
+// Clusters of `size` CTAs (one an SM) that the device runs at once: not every SM of every GPC finds partners.
+uint32_t max_clusters(uint32_t size, int sm_count);
+
 template <int CG>
 Cut cut_of(const MatmulI8Args& m, int sm_count) {
     Cut c{};
@@ -487,10 +498,40 @@ Cut cut_of(const MatmulI8Args& m, int sm_count) {
     c.splits = 1;
     const uint32_t chunks = (m.K + kStep - 1u) / kStep;
     if (CG == 1)
-        while (c.splits < kMaxSplits && c.tiles * c.splits * 2u <= (uint32_t)sm_count && chunks >= c.splits * 8u) c.splits *= 2u;
-    const uint64_t groups = (uint32_t)sm_count / (CG * c.splits), rounds = (c.tiles + groups - 1u) / groups;
+        while (c.splits < kMaxSplits && c.tiles <= max_clusters(c.splits * 2u, sm_count) && chunks >= c.splits * 8u) c.splits *= 2u;
+    const uint64_t groups = CG * c.splits == 1u ? (uint32_t)sm_count : max_clusters(CG * c.splits, sm_count), rounds = (c.tiles + groups - 1u) / groups;
     c.us = (double)rounds * ((chunks + c.splits - 1u) / c.splits) * stage_bytes(c.tile, CG) / 92e3 + (c.splits > 1u ? 1.0 + 0.012 * c.tile : 0.0);
     return c;
+}
+
+uint32_t max_clusters(uint32_t size, int sm_count) {
+    static std::mutex mu;
+    static uint8_t known[KernelConfig::kMaxDevices][4];
+    static KernelConfig kcfg;
+    const void* func = reinterpret_cast<const void*>(matmul_i8_kernel<1, float>);
+    const uint32_t log = size == 2u ? 1u : size == 4u ? 2u : 3u, guess = (uint32_t)sm_count / size;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= KernelConfig::kMaxDevices || kcfg.prepare(func, kThreads, kSmem, nullptr) != cudaSuccess)
+        return guess;
+    std::lock_guard<std::mutex> lock(mu);
+    if (!known[dev][log]) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(guess * size);
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = kSmem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = size, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, func, &cfg) != cudaSuccess || n < 1) {
+            cudaGetLastError();
+            n = (int)guess;
+        }
+        known[dev][log] = (uint8_t)(n < 255 ? n : 255);
+    }
+    return known[dev][log];
 }
 
 template <int CG, typename T>
@@ -500,20 +541,23 @@ cudaError_t launch_tc(const MatmulI8Args& m, const Cut& cut, int sm_count, cudaS
     a.chunks = (m.K + kStep - 1u) / kStep;
     if (cut.tiles > 0x7FFFFFFFull) return cudaErrorInvalidValue;
     a.tile = cut.tile, a.m_tiles = cut.m_tiles, a.tiles = (uint32_t)cut.tiles, a.splits = cut.splits;
-    // (a shorter ring is faster where little else than weights is read: 1 x 128256 x 4096 79 us with 150 KB, 85 with 226)
-    const uint32_t budget = (a.tile <= 48u ? 150u : 226u) * 1024u;
     const uint32_t group = CG == 2 ? 2u : a.splits;
-    a.stages = (budget - smem_bytes(0, a.tile, CG, a.splits)) / stage_bytes(a.tile, CG);
+    // (a shorter ring is faster where little else than weights is read: 1 x 128256 x 4096 79 us with 150 KB, 85 with 226)
+    const uint32_t budget = a.tile <= 48u ? 150u * 1024u : kSmem;
+    // room of its own for the exchange while it is small; else the ring's, for one more hand-shake
+    const bool exchange = a.splits > 1u && a.tile <= 48u;
+    a.in_ring = a.splits > 1u && !exchange;
+    a.stages = (budget - smem_bytes(0, a.tile, CG, exchange)) / stage_bytes(a.tile, CG);
     if (a.stages > kMaxStages) a.stages = kMaxStages;
-    if (a.stages < 2u) return cudaErrorInvalidValue;
+    if (a.stages < 2u || (a.in_ring && a.stages * stage_bytes(a.tile, CG) < exchange_bytes(a.tile))) return cudaErrorInvalidValue;
     a.tmem_cols = 32;
     while (a.tmem_cols < (a.splits > 1u ? 1u : 2u) * a.tile) a.tmem_cols *= 2u;
-    uint32_t groups = (uint32_t)sm_count / group;
-    if (a.splits > 1u || groups > a.tiles) groups = a.tiles;
+    uint32_t groups = group == 1u ? (uint32_t)sm_count : max_clusters(group, sm_count);
+    if (a.splits > 1u || groups > a.tiles) groups = a.tiles;  // (a shared tile is a cluster's only one)
     if (!encode_rows(&a.tmap_w, m.W, m.N, m.K, m.ldw, 128u) || !encode_rows(&a.tmap_x, m.X, m.M, m.K, m.ldx, a.tile / CG)) return cudaErrorInvalidValue;
-    const uint32_t smem = smem_bytes(a.stages, a.tile, CG, a.splits);
+    const uint32_t smem = smem_bytes(a.stages, a.tile, CG, exchange);
     static KernelConfig kcfg;
-    if (cudaError_t e = kcfg.prepare(reinterpret_cast<const void*>(matmul_i8_kernel<CG, T>), kThreads, smem, nullptr)) return e;
+    if (cudaError_t e = kcfg.prepare(reinterpret_cast<const void*>(matmul_i8_kernel<CG, T>), kThreads, kSmem, nullptr)) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(groups * group);
     cfg.blockDim = dim3(kThreads);

@@ -238,7 +238,7 @@ def make_product(M, N, K, seed, with_bias):
 SHAPES = [(1, 1, 1), (1, 7, 15), (1, 1024, 4096), (1, 300, 127), (1, 129, 12289), (2, 128, 128), (3, 1000, 16), (4, 515, 2049), (5, 257, 4096),
           (8, 640, 1024), (9, 130, 8190), (16, 2048, 512), (17, 385, 640), (31, 96, 300), (32, 4096, 4096), (33, 250, 4096), (48, 1024, 1000),
           (64, 128, 4095), (65, 999, 129), (100, 300, 20000), (127, 77, 256), (128, 512, 512), (129, 2000, 768), (200, 1537, 1024),
-          (255, 129, 1000), (256, 256, 4096), (257, 640, 384), (300, 4097, 513), (512, 1024, 2048), (777, 555, 333), (1030, 2305, 640)]
+          (255, 129, 1000), (256, 256, 4096), (130, 300, 4096), (180, 1030, 8200), (250, 4096, 2080), (400, 700, 9000), (257, 640, 384), (300, 4097, 513), (512, 1024, 2048), (777, 555, 333), (1030, 2305, 640)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
