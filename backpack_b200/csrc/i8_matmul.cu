@@ -17,6 +17,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "kernels.h"
 #include "q4k_common.cuh"
 
@@ -505,33 +507,30 @@ Cut cut_of(const MatmulI8Args& m, int sm_count) {
 }
 
 uint32_t max_clusters(uint32_t size, int sm_count) {
-    static std::mutex mu;
-    static uint8_t known[KernelConfig::kMaxDevices][4];
+    static std::atomic<uint32_t> known[KernelConfig::kMaxDevices][4];  // (asked for once: a few calls a product, each some 0.1 us)
     static KernelConfig kcfg;
-    const void* func = reinterpret_cast<const void*>(matmul_i8_kernel<1, float>);
     const uint32_t log = size == 2u ? 1u : size == 4u ? 2u : 3u, guess = (uint32_t)sm_count / size;
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= KernelConfig::kMaxDevices || kcfg.prepare(func, kThreads, kSmem, nullptr) != cudaSuccess)
-        return guess;
-    std::lock_guard<std::mutex> lock(mu);
-    if (!known[dev][log]) {
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(guess * size);
-        cfg.blockDim = dim3(kThreads);
-        cfg.dynamicSmemBytes = kSmem;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = size, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, func, &cfg) != cudaSuccess || n < 1) {
-            cudaGetLastError();
-            n = (int)guess;
-        }
-        known[dev][log] = (uint8_t)(n < 255 ? n : 255);
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= KernelConfig::kMaxDevices) return guess;
+    if (const uint32_t n = known[dev][log].load(std::memory_order_relaxed)) return n;
+    const void* func = reinterpret_cast<const void*>(matmul_i8_kernel<1, float>);
+    if (kcfg.prepare(func, kThreads, kSmem, nullptr) != cudaSuccess) return guess;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(guess * size);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, func, &cfg) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        n = (int)guess;
     }
-    return known[dev][log];
+    known[dev][log].store((uint32_t)n, std::memory_order_relaxed);
+    return (uint32_t)n;
 }
 
 template <int CG, typename T>

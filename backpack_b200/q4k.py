@@ -356,7 +356,7 @@ class Q4KContext:
         torch = self._torch
         if out is None:
             pad = (k + 15) // 16 * 16
-            codes = torch.empty((m, pad), dtype=torch.int8, device=self._dev)
+            codes = torch.empty(m, pad, dtype=torch.int8, device=self._dev)
             scales = torch.empty(m, dtype=torch.float32, device=self._dev)
             return I8Rows(codes if pad == k else codes[:, :k], scales), codes.data_ptr(), scales.data_ptr(), pad
         pc, _, om, ok, ldc = self._rows(out.codes, "codes", torch.int8)
@@ -372,7 +372,7 @@ class Q4KContext:
         ldr = lds = 0
         total = x
         if residual is not None:
-            total = self._torch.empty((m, k), dtype=x.dtype, device=self._dev) if sum_out is None else sum_out
+            total = self._torch.empty(m, k, dtype=x.dtype, device=self._dev) if sum_out is None else sum_out
             pr, _, rm, rk, ldr = self._rows(residual, "residual", x.dtype)
             ps, _, sm, sk, lds = self._rows(total, "sum_out", x.dtype)
             if rm != m or rk != k or sm != m or sk != k:
@@ -414,7 +414,7 @@ class Q4KContext:
         if kw != k:
             raise ValueError(f"x has K={k}, the weight has K={kw}")
         if out is None:
-            out = torch.empty((m, n), dtype=dtype or torch.float32, device=self._dev)
+            out = torch.empty(m, n, dtype=dtype or torch.float32, device=self._dev)
         elif dtype is not None and out.dtype != dtype:
             raise ValueError(f"out is {out.dtype}, not {dtype}")
         py, ft, ym, yn, ldy = self._rows(out, "out")
@@ -436,7 +436,7 @@ class Q4KContext:
             if given.dtype != torch.int32 or given.device != self._dev or given.dim() not in (1, 2) or given.shape[0] != m or not given.is_contiguous():
                 raise ValueError(f"given is not contiguous int32 [{m}] or [{m}, tokens] on {self._dev}")
             g = given.shape[1] if given.dim() == 2 else 1
-            lp = torch.empty(given.shape, dtype=torch.float32, device=self._dev)
+            lp = torch.empty(*given.shape, dtype=torch.float32, device=self._dev)
             if g:
                 pg, plp = given.data_ptr(), lp.data_ptr()
         if not 0 <= top <= LOGPROBS_MAX_TOP:
@@ -444,8 +444,8 @@ class Q4KContext:
         entropy = torch.empty(m, dtype=torch.float32, device=self._dev)
         ids = best = pi = pb = None
         if top:
-            ids = torch.empty((m, top), dtype=torch.int32, device=self._dev)
-            best = torch.empty((m, top), dtype=torch.float32, device=self._dev)
+            ids = torch.empty(m, top, dtype=torch.int32, device=self._dev)
+            best = torch.empty(m, top, dtype=torch.float32, device=self._dev)
             pi, pb = ids.data_ptr(), best.data_ptr()
         st = self.lib.bpq4k_logprobs(self.h, ft, px, m, v, ld, pg, g, plp, entropy.data_ptr(), top, pi, pb, self._stream())
         if st:
