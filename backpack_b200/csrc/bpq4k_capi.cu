@@ -1051,13 +1051,20 @@ int rows_i8(bpq4k_context* h, int ftype, const RowsI8Args& a, cudaStream_t st) {
     if (a.R)
         if (int s = check_rows(h, "residual", a.R, a.K, a.ldr, es)) return s;
     if (a.sum)
+    {
         if (int s = check_rows(h, "sum", a.sum, a.K, a.lds, es)) return s;
+        if ((a.sum == a.X && a.lds != a.ldx) || (a.sum == a.R && a.lds != a.ldr))
+            return fail(h, BPQ4K_ERR_INVALID_ARG, "sum is an input with another distance between rows");
+    }
     if (int s = check_codes(h, "codes", a.codes, a.K, a.ldc)) return s;
     if (int s = check_floats(h, "scales", a.scales)) return s;
     DeviceGuard g(h->device);
     const cudaError_t e = launch_rows_i8(a, ftype, h->sm_count, st);
     h->launches += 1;
-    if (e != cudaSuccess) return cuda_fail(h, e, "8-bit rows launch");
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return cuda_fail(h, e, "8-bit rows launch");
+    }
     return BPQ4K_OK;
 }
 
@@ -1109,7 +1116,10 @@ int bpq4k_matmul_i8(bpq4k_handle_t h, int ftype, const int8_t* X, const float* x
     int launches = 0;
     const cudaError_t e = launch_matmul_i8(a, ftype, h->sm_count, static_cast<cudaStream_t>(stream), &launches);
     h->launches += (uint64_t)launches;
-    if (e != cudaSuccess) return cuda_fail(h, e, "8-bit matmul launch");
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return cuda_fail(h, e, "8-bit matmul launch");
+    }
     return BPQ4K_OK;
 }
 
@@ -1139,7 +1149,10 @@ int bpq4k_logprobs(bpq4k_handle_t h, int ftype, const void* logits, uint32_t M, 
     a.M = M, a.V = V, a.ld = ld, a.nGiven = nGiven, a.nTop = nTop, a.status = h->dev_status;
     const cudaError_t e = launch_logprobs(a, ftype, h->sm_count, static_cast<cudaStream_t>(stream));
     h->launches += 1;
-    if (e != cudaSuccess) return cuda_fail(h, e, "log probability launch");
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return cuda_fail(h, e, "log probability launch");
+    }
     return BPQ4K_OK;
 }
 

@@ -11,6 +11,9 @@
 // Roles (12 warps): warp 0 TMA, warp 1 mma, warp 2 tensor memory, warps 4-11 epilogue.  Persistent over the tiles; two
 // accumulators, so that a tile accumulates while the one before it is stored.
 //
+// A CTA takes more than half of an SM's shared memory, so two that allocate tensor memory never meet on one SM: with kernels on
+// several streams no allocation waits for a CTA that waits in a cluster for a third.
+//
 // Every wait is bounded: on a time-out the role raises the CTA's abort flag and the device status word, waits return at once
 // from then on, copies and mmas in flight are waited for (bounded too), and all threads meet at the end.
 #include <cuda.h>
@@ -501,7 +504,12 @@ Cut cut_of(const MatmulI8Args& m, int sm_count) {
     const uint32_t chunks = (m.K + kStep - 1u) / kStep;
     if (CG == 1)
         while (c.splits < kMaxSplits && c.tiles <= max_clusters(c.splits * 2u, sm_count) && chunks >= c.splits * 8u) c.splits *= 2u;
-    const uint64_t groups = CG * c.splits == 1u ? (uint32_t)sm_count : max_clusters(CG * c.splits, sm_count), rounds = (c.tiles + groups - 1u) / groups;
+    const uint64_t groups = CG * c.splits == 1u ? (uint32_t)sm_count : max_clusters(CG * c.splits, sm_count);
+    if (groups == 0) {  // (a context whose SMs have no partners)
+        c.us = 1e30;
+        return c;
+    }
+    const uint64_t rounds = (c.tiles + groups - 1u) / groups;
     c.us = (double)rounds * ((chunks + c.splits - 1u) / c.splits) * stage_bytes(c.tile, CG) / 92e3 + (c.splits > 1u ? 1.0 + 0.012 * c.tile : 0.0);
     return c;
 }
@@ -512,7 +520,7 @@ uint32_t max_clusters(uint32_t size, int sm_count) {
     const uint32_t log = size == 2u ? 1u : size == 4u ? 2u : 3u, guess = (uint32_t)sm_count / size;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= KernelConfig::kMaxDevices) return guess;
-    if (const uint32_t n = known[dev][log].load(std::memory_order_relaxed)) return n;
+    if (const uint32_t n = known[dev][log].load(std::memory_order_relaxed)) return n - 1u;
     const void* func = reinterpret_cast<const void*>(matmul_i8_kernel<1, float>);
     if (kcfg.prepare(func, kThreads, kSmem, nullptr) != cudaSuccess) return guess;
     cudaLaunchConfig_t cfg{};
@@ -525,11 +533,11 @@ uint32_t max_clusters(uint32_t size, int sm_count) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, func, &cfg) != cudaSuccess || n < 1) {
+    if (cudaOccupancyMaxActiveClusters(&n, func, &cfg) != cudaSuccess || n < 0) {
         cudaGetLastError();
         n = (int)guess;
     }
-    known[dev][log].store((uint32_t)n, std::memory_order_relaxed);
+    known[dev][log].store((uint32_t)n + 1u, std::memory_order_relaxed);
     return (uint32_t)n;
 }
 
@@ -548,7 +556,7 @@ cudaError_t launch_tc(const MatmulI8Args& m, const Cut& cut, int sm_count, cudaS
     a.in_ring = a.splits > 1u && !exchange;
     a.stages = (budget - smem_bytes(0, a.tile, CG, exchange)) / stage_bytes(a.tile, CG);
     if (a.stages > kMaxStages) a.stages = kMaxStages;
-    if (a.stages < 2u || (a.in_ring && a.stages * stage_bytes(a.tile, CG) < exchange_bytes(a.tile))) return cudaErrorInvalidValue;
+    if (a.stages < 2u || smem_bytes(a.stages, a.tile, CG, exchange) <= 114u * 1024u || (a.in_ring && a.stages * stage_bytes(a.tile, CG) < exchange_bytes(a.tile))) return cudaErrorInvalidValue;
     a.tmem_cols = 32;
     while (a.tmem_cols < (a.splits > 1u ? 1u : 2u) * a.tile) a.tmem_cols *= 2u;
     uint32_t groups = group == 1u ? (uint32_t)sm_count : max_clusters(group, sm_count);

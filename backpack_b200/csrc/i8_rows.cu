@@ -284,14 +284,14 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(const __grid_constant__ R
 
 template <typename T, int E, int PT>
 cudaError_t launch_pt(const RowsI8Args& a, cudaStream_t stream) {
-    const uint32_t units = (a.K + PT - 1u) / PT, threads = (units + 31u) & ~31u;
-    if (a.w && a.R)
-        rows_i8_kernel<T, E, PT, true, true><<<a.M, threads, 0, stream>>>(a);
-    else if (a.w)
-        rows_i8_kernel<T, E, PT, true, false><<<a.M, threads, 0, stream>>>(a);
-    else
-        rows_i8_kernel<T, E, PT, false, false><<<a.M, threads, 0, stream>>>(a);
-    return cudaGetLastError();
+    const uint32_t units = (a.K + PT - 1u) / PT;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(a.M);
+    cfg.blockDim = dim3((units + 31u) & ~31u);
+    cfg.stream = stream;
+    if (a.w && a.R) return cudaLaunchKernelEx(&cfg, rows_i8_kernel<T, E, PT, true, true>, a);
+    if (a.w) return cudaLaunchKernelEx(&cfg, rows_i8_kernel<T, E, PT, true, false>, a);
+    return cudaLaunchKernelEx(&cfg, rows_i8_kernel<T, E, PT, false, false>, a);
 }
 
 // Values of a thread.  8: the shortest way through a row, for rows that have an SM each (1 x 4096 float 3.0 us, with 16 3.6), short

@@ -448,7 +448,7 @@ enum bpq4k_ftype { BPQ4K_TYPE_F32 = 0, BPQ4K_TYPE_F16 = 1, BPQ4K_TYPE_BF16 = 30 
 
 /* Residual addition, root-mean-square norm, quantisation; for every row m:
  *     v = X + residual                    in float; residual may be NULL
- *     sum = v                             rounded to the element type; may be NULL, may be X or residual themselves
+ *     sum = v                             rounded to the element type; may be NULL, may be X or residual (same rows)
  *     p = v * weight,  a = max |p|
  *     codes = round(127 p / a)            to the nearest, ties to the even code: the exact quotient, whatever the order of sums
  *     scales = a / sqrt(mean(v^2) + eps) / 127

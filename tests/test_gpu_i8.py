@@ -340,6 +340,7 @@ def test_refusals(ctx):
     assert norm(ft=12) == 2 and norm(K=0) == 2 and norm(K=32769, ldx=40000, ldc=40000) == 2 and norm(M=1 << 31) == 2
     assert norm(x=None) == 1 and norm(w=None) == 1 and norm(c=None) == 1 and norm(s=None) == 1 and norm(sm=y.data_ptr()) == 1
     assert norm(ldx=63) == 1 and norm(ldc=48) == 1 and norm(r=x.data_ptr(), ldr=1) == 1 and norm(r=x.data_ptr(), sm=x.data_ptr(), lds=0) == 1
+    assert norm(r=x.data_ptr(), M=2, sm=x.data_ptr(), lds=128) == 1
     assert norm(eps=-1.0) == 1 and norm(eps=float("nan")) == 1
     assert norm(x=x.data_ptr() + 2) == 3 and norm(c=c.data_ptr() + 8) == 3 and norm(ldc=72) == 3 and norm(s=s.data_ptr() + 1) == 3
     assert "multiple of 16" in (norm(ldc=72), lib.bpq4k_last_error_string(h).decode())[1]
@@ -438,6 +439,104 @@ def test_captured_replayed_and_side_by_side(ctx):
         assert torch.equal(t, wt) and torch.equal(y, wy) and torch.equal(lp.given, wlp.given)
         assert torch.equal(lp.entropy, wlp.entropy) and torch.equal(lp.top_ids, wlp.top_ids) and torch.equal(lp.top, wlp.top)
     assert ctx.device_status() == 0
+
+
+FIRST_CALL_IS_CAPTURED = """
+import torch, backpack_b200 as bp
+ctx = bp.Q4KContext(0)
+g = torch.Generator(device="cuda").manual_seed(1)
+r = lambda *s: torch.randn(*s, device="cuda", generator=g)
+sets = [(r(m, k), r(m, k), torch.rand(k, device="cuda", generator=g), bp.I8Rows(torch.randint(-127, 128, (n, k), dtype=torch.int8, device="cuda", generator=g),
+         torch.rand(n, device="cuda", generator=g))) for m, n, k in [(1, 512, 1024), (20, 512, 8192), (100, 1000, 4096), (300, 2000, 512)]]
+def run(s):
+    rows, total = ctx.add_rmsnorm_i8(s[0], s[2], 1e-5, residual=s[1])
+    y = ctx.matmul_i8(rows, s[3])
+    lp = ctx.logprobs(y, top=3)
+    return total, y, lp.entropy, lp.top_ids
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    outs = [run(s) for s in sets]
+for _ in range(3):
+    graph.replay()
+torch.cuda.synchronize()
+for o, s in zip(outs, sets):
+    assert all(torch.equal(a, b) for a, b in zip(o, run(s)))
+assert ctx.device_status() == 0
+print("captured first")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    import os
+    import subprocess
+    import sys
+
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL_IS_CAPTURED], capture_output=True, text=True, timeout=300,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stderr[-2000:]
+
+
+def test_calls_on_another_stream_and_from_threads(ctx):
+    """Calls queued on a stream that is not the current one's default, a handle per thread."""
+    import threading
+
+    import torch
+
+    sets = [make_last_layer(m, 200 + m) for m in (2, 130)]
+    want = [last_layer(ctx, *s[:3], ctx.quantize_i8(s[3]), s[4]) for s in sets]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        c = Q4KContext(0)
+        try:
+            st = torch.cuda.Stream()
+            with torch.cuda.stream(st):
+                for _ in range(10):
+                    t, y, lp = last_layer(c, *sets[i][:3], c.quantize_i8(sets[i][3]), sets[i][4])
+                    st.synchronize()
+                    if not (torch.equal(y, want[i][1]) and torch.equal(lp.top, want[i][2].top)):
+                        bad.append(i)
+        finally:
+            c.close()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_offsets_beyond_32_bits(ctx):
+    """More than 2^32 codes, values or outputs: the last rows are as they are by themselves."""
+    import torch
+
+    K, N = 32768, 131072 + 300
+    w = I8Rows(torch.empty((N, K), dtype=torch.int8, device="cuda"), torch.rand(N, device="cuda"))
+    for n in range(0, N, 8192):
+        w.codes[n:n + 8192].random_(-127, 128)
+    x = ctx.quantize_i8(torch.randn(200, K, device="cuda"))
+    for m in (1, 20, 200):
+        y = ctx.matmul_i8(x.rows(0, m), w)
+        assert torch.equal(y[:, -500:], ctx.matmul_i8(x.rows(0, m), I8Rows(w.codes[-500:].clone(), w.scales[-500:].clone())))
+        assert torch.equal(y[:, :500], ctx.matmul_i8(x.rows(0, m), w.rows(0, 500)))
+        del y
+    big = I8Rows(w.codes[:, :64].contiguous(), w.scales)
+    xs = I8Rows(torch.empty((33000, 64), dtype=torch.int8, device="cuda").random_(-127, 128), torch.rand(33000, device="cuda"))
+    y = ctx.matmul_i8(xs, big, dtype=torch.bfloat16)                      # 33000 x 131372: 4.3e9 outputs
+    assert torch.equal(y[-3:], ctx.matmul_i8(xs.rows(32997, 33000), big, dtype=torch.bfloat16))
+    given = torch.full((33000,), 131371, dtype=torch.int32, device="cuda")
+    lp = ctx.logprobs(y, given=given, top=2)
+    part = ctx.logprobs(y[-3:].clone(), given=given[-3:], top=2)
+    assert torch.equal(lp.top_ids[-3:], part.top_ids) and torch.allclose(lp.given[-3:], part.given, rtol=1e-5)
+    del y, lp, part
+    v = torch.zeros((N + 8, K), dtype=torch.float16, device="cuda")
+    v[-5:].normal_()
+    got = ctx.quantize_i8(v, out=I8Rows(torch.empty((N + 8, K), dtype=torch.int8, device="cuda"), torch.empty(N + 8, device="cuda")))
+    tail = ctx.quantize_i8(v[-5:].clone())
+    assert torch.equal(got.codes[-5:], tail.codes) and torch.equal(got.scales[-5:], tail.scales) and not bool(got.scales[:-5].any())
 
 
 def test_same_calls_on_the_debug_build():
