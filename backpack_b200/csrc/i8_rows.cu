@@ -10,7 +10,8 @@
 // the exact a.
 //
 // Memory bound (13 bytes a value with a float residual stream).  A row's values stay in registers between the two halves
-// (statistics, codes), one CTA to a row, several rows to an SM, so that one row's loads overlap another's arithmetic.
+// (statistics, codes), one CTA to a row, several rows to an SM, so that one row's loads overlap another's arithmetic; that runs on
+// pairs (.f32x2).  2048 x 8192 float with a residual: 40 us, 0.83 of the copy rate; what is left is the barrier between the halves.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -76,6 +77,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // a NaN if either
 
 constexpr float kNear = 0.5f - 3e-5f;  // a quotient further from its code than this may belong to the next one
 
+constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: added to a quotient, it leaves the rounded quotient in the low byte
+
 // The code of 127 p / peak, which lies in [k, k + 1): on which side of k + 1/2 it is.
 __device__ __forceinline__ uint32_t exact_code(double p, double peak, int k) {
     const double l = 254.0 * p, r = (double)(2 * k + 1) * peak;
@@ -98,23 +101,54 @@ __device__ __forceinline__ void store_codes(int8_t* at, const uint32_t (&q)[E]) 
     }
 }
 
-// A thread holds PT values: PT / E accesses, blockDim.x of them apart; as they were loaded, or (RES) their sums in float.
+// Two floats in a register pair.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// A warp takes 32 * PT neighbouring values of the row, a lane PT / E accesses 32 * E apart, so that all offsets are constants.
+// Values stay as they were loaded, or (RES) as their sums in float; behind the row they are zeros.
 template <typename T, int E, int PT, bool NORM, bool RES>
 __global__ void __launch_bounds__(1024) rows_i8_kernel(const __grid_constant__ RowsI8Args a) {
-    constexpr int NV = PT / E;
+    constexpr int NV = PT / E, G = E == 1 ? 2 : E;  // G: values of a group, which the arithmetic takes in pairs
     const uint32_t row = blockIdx.x, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, warps = blockDim.x >> 5;
-    const T* x = static_cast<const T*>(a.X) + (uint64_t)row * a.ldx;
-    const T* r = RES ? static_cast<const T*>(a.R) + (uint64_t)row * a.ldr : nullptr;
-    T* sum = RES && a.sum ? static_cast<T*>(a.sum) + (uint64_t)row * a.lds : nullptr;
-    int8_t* codes = a.codes + (uint64_t)row * a.ldc;
-
-    auto weights = [&](uint32_t e, float (&w)[E]) {
+    const uint32_t e0 = warp * (32u * PT) + lane * E;
+    const T* x = static_cast<const T*>(a.X) + (uint64_t)row * a.ldx + e0;
+    const T* r = RES ? static_cast<const T*>(a.R) + (uint64_t)row * a.ldr + e0 : nullptr;
+    T* sum = RES && a.sum ? static_cast<T*>(a.sum) + (uint64_t)row * a.lds + e0 : nullptr;
+    int8_t* codes = a.codes + (uint64_t)row * a.ldc + e0;
+    const float* wp = a.w + e0;
+    auto in = [&](int i) { return e0 + (uint32_t)i * (32u * E) < a.K; };
+    auto weights = [&](int g, float (&w)[G]) {  // of group g
         if constexpr (E == 1) {
-            w[0] = __ldg(a.w + e);
+            w[0] = in(2 * g) ? __ldg(wp + 64 * g) : 0.f;
+            w[1] = in(2 * g + 1) ? __ldg(wp + 64 * g + 32) : 0.f;
         } else {
 #pragma unroll
             for (int j = 0; j < E; j += 4) {
-                const float4 t = __ldg(reinterpret_cast<const float4*>(a.w + e + j));
+                const float4 t = in(g) ? __ldg(reinterpret_cast<const float4*>(wp + 32 * E * g + j)) : make_float4(0.f, 0.f, 0.f, 0.f);
                 w[j] = t.x, w[j + 1] = t.y, w[j + 2] = t.z, w[j + 3] = t.w;
             }
         }
@@ -122,39 +156,45 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(const __grid_constant__ R
 
     Pack<T, E> xv[NV] = {};
     float v[RES ? PT : 1] = {};
-    auto value = [&](int i, int j) { return RES ? v[RES ? i * E + j : 0] : to_float(xv[i].v[j]); };
-    float ss = 0.f, hi = 0.f;  // (an infinity or a NaN reaches hi)
+    auto value = [&](int t) { return RES ? v[RES ? t : 0] : to_float(xv[t / E].v[t % E]); };
+    float hi = 0.f;          // (an infinity or a NaN reaches hi)
+    uint64_t ss2 = 0ull;
     {
-        Pack<T, E> rv[RES ? NV : 1];
+        Pack<T, E> rv[RES ? NV : 1] = {};
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const uint32_t e = (tid + i * blockDim.x) * E;
-            if (e < a.K) xv[i] = load_pack<T, E>(x + e);
-        }
+        for (int i = 0; i < NV; i++)
+            if (in(i)) xv[i] = load_pack<T, E>(x + 32 * E * i);
         if constexpr (RES) {
 #pragma unroll
-            for (int i = 0; i < NV; i++) {
-                const uint32_t e = (tid + i * blockDim.x) * E;
-                if (e < a.K) rv[i] = load_pack<T, E>(r + e);
-            }
+            for (int i = 0; i < NV; i++)
+                if (in(i)) rv[i] = load_pack<T, E>(r + 32 * E * i);
         }
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const uint32_t e = (tid + i * blockDim.x) * E;
-            if (e >= a.K) continue;
-            float w[E];
-            if constexpr (NORM) weights(e, w);
+        for (int g = 0; g < PT / G; g++) {
+            float w[G];
+            if constexpr (NORM) weights(g, w);
 #pragma unroll
-            for (int j = 0; j < E; j++) {
-                if constexpr (RES) v[i * E + j] = to_float(xv[i].v[j]) + to_float(rv[i].v[j]);
-                const float s = value(i, j);
-                if constexpr (NORM) ss = fmaf(s, s, ss);
-                hi = max_nan(hi, fabsf(NORM ? s * w[j] : s));
+            for (int j = 0; j < G; j += 2) {
+                const int t = g * G + j;
+                uint64_t s = pair(to_float(xv[t / E].v[t % E]), to_float(xv[(t + 1) / E].v[(t + 1) % E]));
+                if constexpr (RES) {
+                    s = add2(s, pair(to_float(rv[t / E].v[t % E]), to_float(rv[(t + 1) / E].v[(t + 1) % E])));
+                    v[t] = halves(s).x, v[t + 1] = halves(s).y;
+                }
+                if constexpr (NORM) ss2 = fma2(s, s, ss2);
+                const float2 p = halves(NORM ? mul2(s, pair(w[j], w[j + 1])) : s);
+                hi = max_nan(max_nan(hi, fabsf(p.x)), fabsf(p.y));
             }
-            if constexpr (RES)
-                if (sum && BPQ4K_CHECK(e + E <= a.K, a.status)) store_pack<T, E>(sum + e, v + i * E);
+        }
+        if constexpr (RES) {
+            if (sum) {
+#pragma unroll
+                for (int i = 0; i < NV; i++)
+                    if (in(i) && BPQ4K_CHECK(e0 + 32u * E * i + E <= a.K, a.status)) store_pack<T, E>(sum + 32 * E * i, v + i * E);
+            }
         }
     }
+    float ss = halves(ss2).x + halves(ss2).y;
 
     __shared__ uint32_t s_hi[32];
     __shared__ float s_ss[32];
@@ -183,14 +223,12 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(const __grid_constant__ R
             sq = 0.0;
             double big = 0.0;
 #pragma unroll
-            for (int i = 0; i < NV; i++) {
-                const uint32_t e = (tid + i * blockDim.x) * E;
-                if (e >= a.K) continue;
-                float w[E];
-                weights(e, w);
+            for (int g = 0; g < PT / G; g++) {
+                float w[G];
+                weights(g, w);
 #pragma unroll
-                for (int j = 0; j < E; j++) {
-                    const double s = (double)value(i, j);
+                for (int j = 0; j < G; j++) {
+                    const double s = (double)value(g * G + j);
                     sq += s * s;
                     big = fmax(big, fabs(s * (double)w[j]));
                 }
@@ -219,9 +257,8 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(const __grid_constant__ R
     if (zero) {  // (a whole row)
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            const uint32_t e = (tid + i * blockDim.x) * E;
             const uint32_t none[E] = {};
-            if (e < a.K && BPQ4K_CHECK(e + E <= a.K && row < a.M, a.status)) store_codes<E>(codes + e, none);
+            if (in(i) && BPQ4K_CHECK(e0 + 32u * E * i + E <= a.K, a.status)) store_codes<E>(codes + 32 * E * i, none);
         }
         return;
     }
@@ -230,78 +267,87 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(const __grid_constant__ R
     if (NORM && (mine == top || tiny)) {
         double big = 0.0;
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const uint32_t e = (tid + i * blockDim.x) * E;
-            if (e >= a.K) continue;
-            float w[E];
-            weights(e, w);
+        for (int g = 0; g < PT / G; g++) {
+            float w[G];
+            weights(g, w);
 #pragma unroll
-            for (int j = 0; j < E; j++) big = fmax(big, fabs((double)value(i, j) * (double)w[j]));
+            for (int j = 0; j < G; j++) big = fmax(big, fabs((double)value(g * G + j) * (double)w[j]));
         }
         atomicMax(&s_exact, (unsigned long long)__double_as_longlong(big));
     }
     const float inv = tiny ? 0.f : 127.f / peak;
+    const uint64_t inv2 = pair(inv, inv), magic2 = pair(kMagic, kMagic), less2 = pair(-kMagic, -kMagic);
     float far = tiny ? 1.f : 0.f;  // the largest distance of a quotient from its code
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const uint32_t e = (tid + i * blockDim.x) * E;
-        if (e >= a.K) continue;
-        float w[E];
-        if constexpr (NORM) weights(e, w);
-        uint32_t q[E];
+    for (int g = 0; g < PT / G; g++) {
+        float w[G];
+        if constexpr (NORM) weights(g, w);
+        uint32_t q[G];
 #pragma unroll
-        for (int j = 0; j < E; j++) {
-            const float p = NORM ? value(i, j) * w[j] : value(i, j);
-            const float c = fmaf(p, inv, 12582912.f);  // 1.5 * 2^23: the low byte is the rounded quotient
-            q[j] = __float_as_uint(c);
-            far = fmaxf(far, fabsf(fmaf(p, inv, -(c - 12582912.f))));
+        for (int j = 0; j < G; j += 2) {
+            uint64_t p = pair(value(g * G + j), value(g * G + j + 1));
+            if constexpr (NORM) p = mul2(p, pair(w[j], w[j + 1]));
+            const uint64_t c = fma2(p, inv2, magic2);
+            const float2 f = halves(c), n = halves(add2(c, less2)), d = halves(fma2(p, inv2, pair(-n.x, -n.y)));
+            q[j] = __float_as_uint(f.x), q[j + 1] = __float_as_uint(f.y);
+            far = fmaxf(fmaxf(far, fabsf(d.x)), fabsf(d.y));
         }
-        if (BPQ4K_CHECK(e + E <= a.K && row < a.M, a.status)) store_codes<E>(codes + e, q);
+#pragma unroll
+        for (int l = 0; l < G / E; l++) {
+            const int i = g * (G / E) + l;
+            if (in(i) && BPQ4K_CHECK(e0 + 32u * E * i + E <= a.K && row < a.M, a.status))
+                store_codes<E>(codes + 32 * E * i, reinterpret_cast<const uint32_t(&)[E]>(q[l * E]));
+        }
     }
     if constexpr (NORM) __syncthreads();
     if (far > kNear) {
         const double exact = NORM ? __longlong_as_double((long long)s_exact) : (double)peak, by = tiny ? 127.0 / exact : 0.0;
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const uint32_t e = (tid + i * blockDim.x) * E;
-            if (e >= a.K) continue;
-            float w[E];
-            if constexpr (NORM) weights(e, w);
-            uint32_t q[E];
+        for (int g = 0; g < PT / G; g++) {
+            float w[G];
+            if constexpr (NORM) weights(g, w);
+            uint32_t q[G];
 #pragma unroll
-            for (int j = 0; j < E; j++) {
-                const float s = value(i, j), p = NORM ? s * w[j] : s, c = fmaf(p, inv, 12582912.f), d = fmaf(p, inv, -(c - 12582912.f));
+            for (int j = 0; j < G; j++) {
+                const float s = value(g * G + j), p = NORM ? s * w[j] : s, c = fmaf(p, inv, kMagic), d = fmaf(p, inv, -(c - kMagic));
                 q[j] = __float_as_uint(c);
                 if (tiny || fabsf(d) > kNear) {
                     const double pp = NORM ? (double)s * (double)w[j] : (double)s;
-                    q[j] = exact_code(pp, exact, tiny ? (int)floor(pp * by) : __float2int_rn(c - 12582912.f) - (d < 0.f ? 1 : 0));
+                    q[j] = exact_code(pp, exact, tiny ? (int)floor(pp * by) : __float2int_rn(c - kMagic) - (d < 0.f ? 1 : 0));
                 }
             }
-            if (BPQ4K_CHECK(e + E <= a.K && row < a.M, a.status)) store_codes<E>(codes + e, q);
+#pragma unroll
+            for (int l = 0; l < G / E; l++) {
+                const int i = g * (G / E) + l;
+                if (in(i) && BPQ4K_CHECK(e0 + 32u * E * i + E <= a.K && row < a.M, a.status))
+                    store_codes<E>(codes + 32 * E * i, reinterpret_cast<const uint32_t(&)[E]>(q[l * E]));
+            }
         }
     }
 }
 
 template <typename T, int E, int PT>
 cudaError_t launch_pt(const RowsI8Args& a, cudaStream_t stream) {
-    const uint32_t units = (a.K + PT - 1u) / PT;
+    const uint32_t warps = (a.K + 32u * PT - 1u) / (32u * PT);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(a.M);
-    cfg.blockDim = dim3((units + 31u) & ~31u);
+    cfg.blockDim = dim3(warps * 32u);
     cfg.stream = stream;
     if (a.w && a.R) return cudaLaunchKernelEx(&cfg, rows_i8_kernel<T, E, PT, true, true>, a);
     if (a.w) return cudaLaunchKernelEx(&cfg, rows_i8_kernel<T, E, PT, true, false>, a);
     return cudaLaunchKernelEx(&cfg, rows_i8_kernel<T, E, PT, false, false>, a);
 }
 
-// Values of a thread.  8: the shortest way through a row, for rows that have an SM each (1 x 4096 float 3.0 us, with 16 3.6), short
-// rows (2048 x 768 float 6.3 against 7.0) and single accesses (2048 x 5001 half 56 against 67).  16: more loads in flight per SM
-// (2048 x 8192 float 38.7 us, with 8 48.3, with 32 53.9; bfloat16 30.1, 39.7, 33.4).  32: rows that need it, and 16-bit rows
-// without a residual from 8192 on, whose values stay packed (512 x 14336 bfloat16 12.5 us, with 16 13.8).
+// Values of a thread (us on B200; R: with a residual).  8: the shortest way through a row, for rows that have an SM each (1 x 4096
+// float R 3.2, with 16 3.4) and short rows (2048 x 768 float R 5.8, 7.2; 2048 x 1025 bfloat16 R, single accesses, 8.1, 9.6).  32:
+// most loads in flight per SM, for long rows and many (2048 x 8192 float R 39.9, with 16 42.0, with 8 46.6; bfloat16 R 26.8, 29.0,
+// 37.7; 2048 x 14336 float R 65.6, 74.1), but not with single accesses, whose 32 of each operand spill (2048 x 5001 half R 37.9,
+// with 16 22.8).  16: between (200 x 8192 float R 7.2, with 8 8.0, with 32 8.7; 4096 x 2048 bfloat16 R 14.4, 15.3, 15.6).
 template <typename T, int E>
 cudaError_t launch_vec(const RowsI8Args& a, int sm_count, cudaStream_t stream) {
-    if (a.K <= 8192u && (a.M <= (uint32_t)sm_count || a.K <= 1024u || E == 1)) return launch_pt<T, E, 8>(a, stream);
-    if (a.K <= 8192u || (a.K <= 16384u && (sizeof(T) == 4 || a.R))) return launch_pt<T, E, 16>(a, stream);
+    const uint32_t sms = (uint32_t)sm_count;
+    if (a.K <= 8192u && (a.M <= sms || a.K <= (E == 1 ? 2048u : 1024u))) return launch_pt<T, E, 8>(a, stream);
+    if (a.K <= 16384u && (E == 1 || a.K <= 4096u || a.M <= 2u * sms)) return launch_pt<T, E, 16>(a, stream);
     return launch_pt<T, E, 32>(a, stream);
 }
 
