@@ -15,6 +15,10 @@
 // against 54).
 //
 // Few rows: CTAs of a cluster share a row, so that no working memory is needed; the first of them gathers.
+//
+// What bounds it.  Float logits: DRAM (512 x 128256: 42 us without alternatives, 0.95 of the copy rate; 48 with five: a row's last
+// 5 us, the selection, have no other row to overlap).  16-bit logits: instructions, about 11 a value (32 us, 0.63; the exponentials
+// alone are 15).  Few rows: the chain load, reduce, select, gather (1 x 128256: 4.9 us, with 20 alternatives 9.6).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -31,7 +35,6 @@ namespace {
 constexpr uint32_t kFull = 0xFFFFFFFFu;
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint32_t kBlocks = 1024;       // blocks whose maxima are kept
 constexpr uint32_t kBlockValues = 1024;  // values of a step, and of the smallest block that is not fine
 constexpr uint32_t kMaxGroup = 8;  // CTAs that share a row: the largest cluster that every device takes
 
@@ -107,24 +110,18 @@ __device__ __forceinline__ float largest(const uint4 (&p)[U], T) {
 // Maximum, S and T of some values, T in units of ln 2.
 struct Stats {
     float m, s, t;
-    __device__ __forceinline__ void add(const Stats& o) {
-        const float n = max_nan(m, o.m);
-        // (-infinity less -infinity is a NaN, and fmaxf drops it; 2^-300 is 0 as a float)
-        const float d = fmaxf((m - n) * kLog2e, -300.f), od = fmaxf((o.m - n) * kLog2e, -300.f);
-        const float f = exp2_fast(d), of = exp2_fast(od);
-        t = f * fmaf(s, d, t) + of * fmaf(o.s, od, o.t);
-        s = s * f + o.s * of;
-        m = n;
-    }
-    __device__ __forceinline__ void add_lanes() {  // over the warp; the result is lane 0's
-#pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            const Stats other{__shfl_down_sync(kFull, m, o), __shfl_down_sync(kFull, s, o), __shfl_down_sync(kFull, t, o)};
-            add(other);
-        }
-        m = __shfl_sync(kFull, m, 0), s = __shfl_sync(kFull, s, 0), t = __shfl_sync(kFull, t, 0);
-    }
 };
+// The sum of the first n lanes' (n a power of two), in all lanes.
+__device__ __forceinline__ Stats add_lanes(Stats v, uint32_t n) {
+    float m = v.m;
+    for (uint32_t o = n >> 1; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(kFull, m, o));
+    // (-infinity less -infinity is a NaN, and fmaxf drops it; 2^-300 is 0 as a float)
+    const float d = fmaxf((v.m - m) * kLog2e, -300.f), f = exp2_fast(d);
+    v.t = f * fmaf(v.s, d, v.t);
+    v.s *= f;
+    for (uint32_t o = n >> 1; o; o >>= 1) v.s += __shfl_xor_sync(kFull, v.s, o), v.t += __shfl_xor_sync(kFull, v.t, o);
+    return {__shfl_sync(kFull, m, 0), __shfl_sync(kFull, v.s, 0), __shfl_sync(kFull, v.t, 0)};
+}
 
 __device__ __forceinline__ unsigned long long make_key(float v, uint32_t idx) {
     const uint32_t b = __float_as_uint(v + 0.f);  // (-0 and +0 are equal)
@@ -148,41 +145,18 @@ __device__ __forceinline__ void store_cluster(V* at, const V& v) {
     for (uint32_t i = 0; i < sizeof(V) / 4; i++) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + 4u * i), "r"(w[i]) : "memory");
 }
 
-// Keys of a warp in descending order over its lanes.
-__device__ __forceinline__ unsigned long long sort_warp(unsigned long long k, uint32_t lane) {
-#pragma unroll
-    for (uint32_t size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (uint32_t step = size >> 1; step; step >>= 1) {
-            const unsigned long long o = __shfl_xor_sync(kFull, k, step);
-            const bool larger = ((lane & step) == 0u) == ((lane & size) == 0u || size == 32u);
-            k = (k > o) == larger ? k : o;
-        }
-    return k;
-}
-// The best 32 of two descending lists of 32, descending.
-__device__ __forceinline__ unsigned long long merge_warp(unsigned long long a, unsigned long long b, uint32_t lane) {
-    const unsigned long long r = __shfl_sync(kFull, b, 31u - lane);
-    unsigned long long k = a > r ? a : r;
-#pragma unroll
-    for (uint32_t step = 16; step; step >>= 1) {
-        const unsigned long long o = __shfl_xor_sync(kFull, k, step);
-        k = (k > o) == ((lane & step) == 0u) ? k : o;
+// How many of n keys are larger than `mine`; keys[n] may be read and is 0 where n is odd.  All keys differ, so this is the key's
+// place in descending order: for the few hundred keys here, reads that do not wait for one another, where a sort is a chain of
+// exchanges (lists of the warps, sorted and merged in a tree: 8 x 128256, 5 tokens 8.5 us, by places 8.1; 512 x 4000 7.9, 7.3;
+// only 1 x 128256, 20 tokens 8.8, 9.6).
+__device__ __forceinline__ uint32_t place_of(const unsigned long long* keys, uint32_t n, unsigned long long mine) {
+    uint32_t place = 0;
+#pragma unroll 8
+    for (uint32_t i = 0; i < n; i += 2u) {
+        const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(keys + i);
+        place += (k.x > mine ? 1u : 0u) + (k.y > mine ? 1u : 0u);
     }
-    return k;
-}
-
-// The best 32 of the lists of all warps, in every warp's `list`.  keys: 32 per warp; the whole CTA comes here.
-template <uint32_t WARPS>
-__device__ __forceinline__ unsigned long long merge_cta(unsigned long long list, unsigned long long (*keys)[32], uint32_t warp, uint32_t lane) {
-    keys[warp][lane] = list;
-#pragma unroll
-    for (uint32_t step = WARPS / 2u; step; step >>= 1) {
-        __syncthreads();
-        if (warp < step) keys[warp][lane] = list = merge_warp(list, keys[warp + step][lane], lane);
-    }
-    __syncthreads();
-    return keys[0][lane];
+    return place;
 }
 
 // FINE: a block is one access of a warp, else a step or more.
@@ -208,13 +182,14 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
     uint32_t single = a.V;
     if (rank == 0 && tid < head) single = tid;
     if (rank == group - 1u && tid >= 32u && tail + tid - 32u < a.V) single = tail + tid - 32u;
-    // lines of 32 accesses; 2^shift of them are a block, as few as the blocks' maxima have room for
+    // lines of 32 accesses; 2^shift of them are a block
     constexpr uint32_t kStep = 32u * U;
     const uint32_t steps = (v1 - v0 + kStep - 1u) / kStep, lines = (v1 - v0 + 31u) / 32u;
     uint32_t shift = FINE ? 0u : kLog;
-    while ((lines >> shift) >= kBlocks) shift++;
+    while (!FINE && (lines >> shift) >= kThreads) shift++;  // a thread to a block; fine ones are few enough (launch_type)
     const uint32_t blocks = (lines + (1u << shift) - 1u) >> shift;
-    __shared__ float s_block[TOP ? kBlocks : 1];
+    __shared__ __align__(16) unsigned long long s_keys[TOP ? kThreads : 1];  // of the blocks: the largest value, the position
+    if (TOP && tid >= blocks) s_keys[tid] = 0ull;
 
     // the given tokens' logits, the first of each thread: fetched now, needed at the end
     int32_t id = -1;
@@ -266,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
                     const uint4 one[1] = {p[u]};
                     const float line = warp_max_nan(i + 32u * u < v1 ? largest<1>(one, T(0.f)) : -kInf);
                     mx = max_nan(mx, line);
-                    if (TOP && FINE && lane == 0 && step * U + u < lines && BPQ4K_CHECK(lines <= kBlocks, a.status)) s_block[step * U + u] = line;
+                    if (TOP && FINE && lane == 0 && step * U + u < lines && BPQ4K_CHECK(lines <= kThreads, a.status)) s_keys[step * U + u] = make_key(line, step * U + u);
                 }
             }
             if (!(mx <= m)) raise(max_nan(mx, m));
@@ -275,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
             for (uint32_t u = 0; u < U; u++)
                 if (whole || i + 32u * u < v1) take_access(p[u]);
         }
-        if (TOP && !FINE && lane == 0 && BPQ4K_CHECK(b < blocks, a.status)) s_block[b] = block;
+        if (TOP && !FINE && lane == 0 && BPQ4K_CHECK(b < kThreads, a.status)) s_keys[b] = make_key(block, b);
     }
     if (warp < 2u) {
         const float v = single < a.V ? to_float(x[single]) : -kInf, mx = warp_max_nan(v);
@@ -284,28 +259,30 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
     }
     Stats st{m, halves(s2).x + halves(s2).y, halves(t2).x + halves(t2).y};
 
-    __shared__ unsigned long long s_keys[kWarps][32];
     __shared__ Stats s_stats[kWarps];
-    __shared__ unsigned long long s_found[TOP ? kThreads : 1];
+    __shared__ __align__(16) unsigned long long s_found[TOP ? kThreads : 1];
+    __shared__ unsigned long long s_list[32];  // the first blocks, then the largest keys, in descending order; 0 behind the last
     __shared__ uint32_t s_count;
-    __shared__ unsigned long long c_keys[TOP ? kMaxGroup : 1][32];
+    __shared__ __align__(16) unsigned long long c_keys[TOP ? kMaxGroup * 32u : 1];
     __shared__ Stats c_stats[kMaxGroup];
-    st.add_lanes();
+#pragma unroll
+    for (int o = 16; o; o >>= 1) st.s += __shfl_xor_sync(kFull, st.s, o), st.t += __shfl_xor_sync(kFull, st.t, o);  // (one maximum a warp)
     if (lane == 0) s_stats[warp] = st;
-    unsigned long long list = 0ull;
     if constexpr (TOP) {
+        if (tid < 32u) s_list[tid] = 0ull;
         __syncthreads();
-        // the k first blocks: lane i has the i-th
-        unsigned long long best = 0ull;
-        for (uint32_t b = warp * 32u; b < blocks; b += kThreads) {
-            const unsigned long long k = sort_warp(b + lane < blocks ? make_key(s_block[b + lane], b + lane) : 0ull, lane);
-            best = b < kThreads ? k : merge_warp(best, k, lane);
+        // the k first blocks
+        const unsigned long long own = s_keys[tid];
+        if (own) {
+            const uint32_t place = place_of(s_keys, blocks, own);
+            if (place < a.nTop) s_list[place] = own;
         }
-        best = merge_cta<kWarps>(best, s_keys, warp, lane);
-        const unsigned long long bound = __shfl_sync(kFull, best, a.nTop - 1u);
+        __syncthreads();
+        const unsigned long long best = s_list[lane], bound = s_list[a.nTop - 1u];
         // what a key has to exceed: the k-th block has a value like its largest, at its end if nowhere else
         unsigned long long least = 0ull;
         if (bound) least = make_key(key_value(bound), head + min(v1, v0 + ((key_index(bound) + 1u) << shift) * 32u) * E - 1u) - 1ull;
+        const uint32_t first_lines = __popc(__ballot_sync(kFull, best != 0ull)) << shift;  // (lane i has the i-th block; none behind the k-th)
         // Keys above `least` are collected, a few more than k as a rule.  Should they not fit, the k-th of those that did is a better
         // bound, and the blocks are read again.
         for (;;) {
@@ -317,54 +294,62 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
                 const uint32_t at = atomicAdd(&s_count, 1u);
                 if (at < kThreads) s_found[at] = k;
             };
-            for (uint32_t w = warp; w < a.nTop; w += kWarps) {
-                const unsigned long long k = __shfl_sync(kFull, best, w);
-                if (k == 0ull) break;
-                const uint32_t b = key_index(k);
-                constexpr uint32_t R = FINE ? 1u : 4u;
-                for (uint32_t line = b << shift; line < min(lines, (b + 1u) << shift); line += R) {
-                    const uint32_t i = v0 + line * 32u + lane;
-                    uint4 p[R];
+            // the lines of the blocks, dealt to the warps, R of each in flight
+            constexpr uint32_t R = 4;
+            for (uint32_t l0 = warp; l0 < first_lines; l0 += R * kWarps) {
+                uint4 p[R];
+                uint32_t at[R];
 #pragma unroll
-                    for (uint32_t u = 0; u < R; u++)
-                        if (BPQ4K_CHECK(line < lines, a.status) && i + 32u * u < v1) p[u] = __ldg(xv + i + 32u * u);
-#pragma unroll
-                    for (uint32_t u = 0; u < R; u++)
-#pragma unroll
-                        for (uint32_t j = 0; j < E; j++)
-                            if (i + 32u * u < v1) offer(make_key(to_float(reinterpret_cast<const T*>(&p[u])[j]), head + (i + 32u * u) * E + j));
+                for (uint32_t u = 0; u < R; u++) {
+                    const uint32_t l = l0 + u * kWarps, b = key_index(__shfl_sync(kFull, best, min(l >> shift, 31u)));
+                    at[u] = v1;
+                    if (l < first_lines) at[u] = v0 + ((b << shift) + (l & ((1u << shift) - 1u))) * 32u + lane;
+                    if (BPQ4K_CHECK(l >= first_lines || b < blocks, a.status) && at[u] < v1) p[u] = __ldg(xv + at[u]);
                 }
+#pragma unroll
+                for (uint32_t u = 0; u < R; u++)
+#pragma unroll
+                    for (uint32_t j = 0; j < E; j++)
+                        if (at[u] < v1) offer(make_key(to_float(reinterpret_cast<const T*>(&p[u])[j]), head + at[u] * E + j));
             }
             if (single < a.V) offer(make_key(to_float(x[single]), single));
             __syncthreads();
-            const uint32_t found = s_count;
-            list = s_found[tid];
-            if (found > 32u || warp == 0) list = sort_warp(list, lane);
-            if (found > 32u) list = merge_cta<kWarps>(list, s_keys, warp, lane);
-            if (found <= kThreads) break;
-            least = __shfl_sync(kFull, list, a.nTop - 1u) - 1ull;
+            const uint32_t found = s_count, kept = min(found, kThreads);
+            const unsigned long long key = s_found[tid];
+            if (tid < 32u) s_list[tid] = 0ull;
             __syncthreads();
+            if (key) {
+                const uint32_t place = place_of(s_found, kept, key);
+                if (place < 32u) s_list[place] = key;
+            }
+            __syncthreads();
+            if (found <= kThreads) break;
+            least = s_list[a.nTop - 1u] - 1ull;
         }
-        __syncthreads();
     } else {
         __syncthreads();
     }
-    st = lane < kWarps ? s_stats[lane] : Stats{-kInf, 0.f, 0.f};
-    st.add_lanes();
+    st = add_lanes(s_stats[lane % kWarps], kWarps);
     if (group > 1u) {
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (warp == 0) {
-            if constexpr (TOP) store_cluster(&c_keys[rank][lane], list);
+            if (TOP && lane < a.nTop) store_cluster(&c_keys[rank * a.nTop + lane], s_list[lane]);
             if (lane == 0) store_cluster(&c_stats[rank], st);
         }
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (rank) return;
-        st = lane < group ? c_stats[lane] : Stats{-kInf, 0.f, 0.f};
-        st.add_lanes();
+        st = add_lanes(c_stats[lane % group], group);
         if constexpr (TOP) {
-            list = c_keys[0][lane];
-            for (uint32_t g = 1; g < group; g++) list = merge_warp(list, c_keys[g][lane], lane);
+            if (tid < 32u) s_list[tid] = 0ull;
+            __syncthreads();
+            for (uint32_t i = tid; i < group * a.nTop; i += kThreads) {  // (an even number: clusters are)
+                const unsigned long long key = c_keys[i];
+                if (key == 0ull) continue;
+                const uint32_t place = place_of(c_keys, group * a.nTop, key);
+                if (place < a.nTop) s_list[place] = key;
+            }
+            __syncthreads();
         }
     }
     const bool bad = !(st.m < kInf);      // a NaN or +infinity
@@ -379,8 +364,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
         a.given_lp[(uint64_t)row * a.nGiven + g] = is_token(id) ? logp(to_float(x[id])) : nan;
     }
     if (TOP && tid < a.nTop) {
-        a.top_ids[(uint64_t)row * a.nTop + tid] = bad ? -1 : (int32_t)key_index(list);
-        a.top_lp[(uint64_t)row * a.nTop + tid] = logp(key_value(list));
+        const unsigned long long key = s_list[tid];
+        a.top_ids[(uint64_t)row * a.nTop + tid] = bad ? -1 : (int32_t)key_index(key);
+        a.top_lp[(uint64_t)row * a.nTop + tid] = logp(key_value(key));
     }
 }
 
@@ -404,8 +390,8 @@ cudaError_t launch_type(const LogprobsArgs& a, int sm_count, cudaStream_t stream
     uint32_t group = 1;
     while (group < kMaxGroup && (uint64_t)a.M * group * 2u <= 4ull * sm_count && a.V >= group * 2u * 4096u) group *= 2u;
     if (!a.nTop) return launch_rows<T, false, false, 256>(a, group, stream);
-    // fine blocks where there are too few of the others for the most that can be asked of a CTA's part of a row
-    if (a.V / group >= kLogprobsMaxTop * kBlockValues) return launch_rows<T, true, false, 256>(a, group, stream);
+    // fine blocks where a CTA's part of a row has fewer of the others than tokens are asked for
+    if (a.V / group >= a.nTop * kBlockValues) return launch_rows<T, true, false, 256>(a, group, stream);
     // (512 x 4000 float: 128 threads 7.7 us, 256 8.7; 8 x 128256, eight CTAs a row: 11.0 and 9.0)
     if (a.V / group > 4096u) return launch_rows<T, true, true, 256>(a, group, stream);
     return launch_rows<T, true, true, 128>(a, group, stream);

@@ -71,7 +71,7 @@ def check(ctx, x, given, k):
 
 
 SHAPES = [(1, 1), (1, 2), (2, 5), (3, 31), (2, 33), (1, 511), (4, 513), (2, 1000), (1, 4099), (5, 8192), (7, 20011), (1, 32003), (3, 32000), (1, 128256),
-          (2, 131072), (40, 3001), (300, 1031), (1000, 70)]
+          (2, 131072), (40, 3001), (600, 32767), (160, 32768), (3, 262144 + 5), (2, 1100003), (300, 1031), (1000, 70)]
 
 
 @pytest.mark.parametrize("kind", TYPES)
