@@ -425,26 +425,38 @@ __global__ void __launch_bounds__(kThreads, 2) matmul_i8_kernel(const __grid_con
                     if (e < a.splits) mbar_arrive_cluster(peer_addr(ready_bar, e));
                     ready = wait_bar(ready_bar, 0u, abort_flag, a.status) && ok;
                 }
-                for (uint32_t c = side * 8u; c < cols && ready; c += 16u) {
-                    uint32_t v[8];
-                    tmem_ld8(acc + c, v);
+                // (tiles of 16 columns: eight to either side)
+                auto send = [&](uint32_t c, const uint32_t* v, uint32_t n) {
 #pragma unroll
-                    for (uint32_t j = 0; j < 8; j++)
+                    for (uint32_t j = 0; j < n; j++)
                         if (c + j < cols)
                             asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_addr(slot + ((c + j) >> log) * 512u, j & mask)), "r"(v[j]) : "memory");
+                };
+                if (a.tile == 16u) {
+                    uint32_t v[8];
+                    if (ready) tmem_ld8(acc + side * 8u, v), send(side * 8u, v, 8u);
+                } else {
+                    for (uint32_t c = side * 16u; c < cols && ready; c += 32u) {
+                        uint32_t v[16];
+                        tmem_ld16(acc + c, v);
+                        send(c, v, 16u);
+                    }
                 }
                 asm volatile("fence.acq_rel.cluster;" ::: "memory");
                 __syncwarp();
                 if (lane < a.splits) mbar_arrive_cluster(peer_addr(parts_bar, lane));
                 const bool all = wait_bar(parts_bar, 0u, abort_flag, a.status);
                 const int* parts = reinterpret_cast<const int*>(base_ptr + off_exchange) + r;
-                for (uint32_t c = side; part + (c << log) < cols && all && live; c += 2u) {
-                    int sum = 0;
+                if (all && live) {
+#pragma unroll 4
+                    for (uint32_t c = side; part + (c << log) < cols; c += 2u) {
+                        int sum = 0;
 #pragma unroll
-                    for (uint32_t p = 0; p < kMaxSplits; p++)
-                        if (p < a.splits) sum += parts[(p * cols_each + c) * 128u];
-                    const uint32_t m = part + (c << log);
-                    Y[(uint64_t)(m0 + m) * a.ldy + n] = to_elem<T>(finish(sum, xscale[m], wscale, bias));
+                        for (uint32_t p = 0; p < kMaxSplits; p++)
+                            if (p < a.splits) sum += parts[(p * cols_each + c) * 128u];
+                        const uint32_t m = part + (c << log);
+                        Y[(uint64_t)(m0 + m) * a.ldy + n] = to_elem<T>(finish(sum, xscale[m], wscale, bias));
+                    }
                 }
             }
         }
