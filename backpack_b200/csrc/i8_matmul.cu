@@ -407,7 +407,8 @@ __global__ void __launch_bounds__(kThreads, 2) matmul_i8_kernel(const __grid_con
             float* xscale = scale + buf * kMaxTile;
             if (e < cols) xscale[e] = __ldg(a.xs + m0 + e);
             epilogue_sync();
-            const bool ok = wait_bar(acc_full(buf), (i >> 1) & 1u, abort_flag, a.status);
+            // (a whole warp reads tensor memory, or none of it)
+            const bool ok = __all_sync(0xFFFFFFFFu, wait_bar(acc_full(buf), (i >> 1) & 1u, abort_flag, a.status));
             fence_after();
             const uint32_t acc = tmem + ((quad * 32u) << 16) + buf * a.tile;
             if (CG == 2 || a.splits == 1u) {
@@ -450,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 2) matmul_i8_kernel(const __grid_con
                 bool ready = ok;
                 if (a.in_ring) {  // this CTA's mmas are done with its ring; the others'?
                     if (e < a.splits) mbar_arrive_cluster(peer_addr(ready_bar, e));
-                    ready = wait_bar(ready_bar, 0u, abort_flag, a.status) && ok;
+                    ready = __all_sync(0xFFFFFFFFu, wait_bar(ready_bar, 0u, abort_flag, a.status)) && ok;
                 }
                 // (tiles of 16 columns: eight to either side)
                 auto send = [&](uint32_t c, const uint32_t* v, uint32_t n) {
