@@ -372,7 +372,7 @@ class Q4KContext:
         ldr = lds = 0
         total = x
         if residual is not None:
-            total = self._torch.empty(m, k, dtype=x.dtype, device=self._dev) if sum_out is None else sum_out
+            total = self._torch.empty(*x.shape, dtype=x.dtype, device=self._dev) if sum_out is None else sum_out
             pr, _, rm, rk, ldr = self._rows(residual, "residual", x.dtype)
             ps, _, sm, sk, lds = self._rows(total, "sum_out", x.dtype)
             if rm != m or rk != k or sm != m or sk != k:

@@ -302,6 +302,23 @@ def test_matmul_result_does_not_depend_on_the_batch(ctx):
         assert torch.equal(ctx.matmul_i8(xr.rows(0, m), wr, bias=bias), whole[:m]), m
 
 
+def test_rows_of_several_dimensions(ctx):
+    """[batch, tokens, K] and a single row [K] are rows like any others."""
+    import torch
+
+    x, r = torch.randn(3, 5, 256, device="cuda"), torch.randn(3, 5, 256, device="cuda")
+    w = torch.rand(256, device="cuda")
+    got, total = ctx.add_rmsnorm_i8(x, w, 1e-5, residual=r)
+    flat, flat_total = ctx.add_rmsnorm_i8(x.view(15, 256), w, 1e-5, residual=r.view(15, 256))
+    assert total.shape == x.shape and torch.equal(total.view(15, 256), flat_total) and torch.equal(got.codes, flat.codes)
+    one, one_total = ctx.add_rmsnorm_i8(x[1, 2], w, 1e-5, residual=r[1, 2])
+    assert torch.equal(one.codes[0], flat.codes[7]) and torch.equal(one_total, flat_total[7])
+    assert torch.equal(ctx.quantize_i8(x).codes, ctx.quantize_i8(x.view(15, 256)).codes)
+    head = ctx.quantize_i8(torch.randn(40, 256, device="cuda"))
+    out = torch.empty(3, 5, 40, device="cuda")
+    assert ctx.matmul_i8(got, head, out=out) is out and torch.equal(out.view(15, 40), ctx.matmul_i8(flat, head))
+
+
 def test_nothing_to_do(ctx):
     import torch
 
