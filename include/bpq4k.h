@@ -454,7 +454,7 @@ enum bpq4k_ftype { BPQ4K_TYPE_F32 = 0, BPQ4K_TYPE_F16 = 1, BPQ4K_TYPE_BF16 = 30 
  *     scales = a / sqrt(mean(v^2) + eps) / 127
  * so that codes * scales is the norm's output.  A row of zeros has codes and scale 0.  A row in which a value or a product is
  * infinite or not a number has codes 0 and a NaN as its scale, which reaches everything that is made of it.  1 <= K <= 32768.
- * Replaces add_rms_norm and the activation side of the Q8 dispatches (runtime/model_runner.cpp:3200-3243). */
+ * Replaces add_rms and the activation side of the Q8 dispatches (runtime/model_runner.cpp:3200-3243). */
 int bpq4k_add_rmsnorm_i8(bpq4k_handle_t h, int ftype, const void* X, const void* residual, const float* weight, float eps,
                          void* sum, int8_t* codes, float* scales, uint32_t M, uint32_t K, uint32_t ldx, uint32_t ldr,
                          uint32_t lds, uint32_t ldc, void* stream);
