@@ -302,6 +302,27 @@ def test_matmul_result_does_not_depend_on_the_batch(ctx):
         assert torch.equal(ctx.matmul_i8(xr.rows(0, m), wr, bias=bias), whole[:m]), m
 
 
+@pytest.mark.parametrize("name,bits", [("bfloat16", 8), ("float16", 11)])
+def test_every_16_bit_quotient(ctx, name, bits):
+    """Each row has another mantissa n as its largest value, n * 2^-10, and all mantissas m, m * 2^-10-t for t = 0 .. 8, below it:
+    codes round_half_even(127 m / (n 2^t)) in whole numbers."""
+    import torch
+
+    dtype, low, high = getattr(torch, name), 1 << (bits - 1), 1 << bits
+    m, t = (a.reshape(1, -1) for a in np.meshgrid(np.arange(low, high), np.arange(9), indexing="ij"))
+    n = np.arange(low, high).reshape(-1, 1)
+    m = np.where((t == 0) & (m > n), n, m)
+    x = torch.from_numpy(m * 0.5 ** (10 + t)).to(dtype)
+    assert torch.equal(x.double(), torch.from_numpy(m * 0.5 ** (10 + t)))
+    x[:, ::3] *= -1
+    got = ctx.quantize_i8(x.cuda()).codes.cpu().numpy()
+    num, den = 127 * m, n << t
+    k, rest = num // den, 2 * (num % den)
+    want = np.where((rest > den) | ((rest == den) & (k % 2 == 1)), k + 1, k)
+    want[:, ::3] *= -1
+    np.testing.assert_array_equal(got, want)
+
+
 def test_rows_of_several_dimensions(ctx):
     """[batch, tokens, K] and a single row [K] are rows like any others."""
     import torch
