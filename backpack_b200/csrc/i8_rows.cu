@@ -12,11 +12,12 @@
 // p = m 2^-t and a = n (whole mantissas of at most 11 bits), a quotient is a border or at least 2^-12 2^-t away from one, and a float's
 // error is below 254 * 2^-23 * 2^-t: only exact borders can go wrong, 254 m = (2k+1) n 2^t.  127 divides 2k+1 or n.  If not n, k = 63,
 // and 127/a rounded up makes that 64 (the even code), so a multiply-add is all there is to a code.  If n, as above (one row in 64).
-// 2048 x 14336 bfloat16 31.3 -> 21.3 us, 512 x 14336 11.9 -> 10.1: a third of the warps' instructions were borders.
+// Almost half of the warps' instructions went into borders before (2048 x 14336 bfloat16 31.3 us, now 20.9).
 //
 // Memory bound (13 bytes a value with a float residual stream).  A row's values stay in registers between the two halves
 // (statistics, codes), one CTA to a row, several rows to an SM, so that one row's loads overlap another's arithmetic; that runs on
-// pairs (.f32x2).  2048 x 8192 float with a residual: 40 us, 0.83 of the copy rate; what is left is the barrier between the halves.
+// pairs (.f32x2).  2048 x 8192 float with a residual: 35 us, 0.95 of the copy rate.  With 16-bit streams instructions bound it, some 20 a
+// value (bfloat16 27 us, 0.66).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -135,8 +136,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 
 // A warp takes 32 * PT neighbouring values of the row, a lane PT / E accesses 32 * E apart, so that all offsets are constants.
 // Values stay as they were loaded, or (RES) as their sums in float; behind the row they are zeros.
+// Without a norm, 32 registers a thread, for twice the warps (2048 x 8192 float 14.8 us, 512 x 14336 bfloat16 8.1, with up to 64
+// 10.1; not for 32 floats in accesses of 16 bytes, which spill: 512 x 28672 float 23.4, with 64 17.5).  With one there is no gain
+// in fewer (2048 x 8192 float with a residual 40.6 us with 40, 34.9 with 64).
 template <typename T, int E, int PT, bool NORM, bool RES>
-__global__ void __launch_bounds__(1024) rows_i8_kernel(const __grid_constant__ RowsI8Args a) {
+__global__ void __launch_bounds__(1024, NORM || (PT == 32 && E == 4) ? 1 : 2) rows_i8_kernel(const __grid_constant__ RowsI8Args a) {
     constexpr int NV = PT / E, G = E == 1 ? 2 : E;  // G: values of a group, which the arithmetic takes in pairs
     const uint32_t row = blockIdx.x, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, warps = blockDim.x >> 5;
     const uint32_t e0 = warp * (32u * PT) + lane * E;
@@ -268,8 +272,45 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(const __grid_constant__ R
         return;
     }
 
+    if constexpr (!NORM) {
+        constexpr bool kShort = sizeof(T) == 2;  // (with 127 no divisor of the mantissa of a)
+        bool exactly = tiny || (kShort && ((top & 0x7FFFFFu) | 0x800000u) % 127u == 0u);
+        if (!exactly) {
+            const float inv = kShort ? __fdiv_ru(127.f, peak) : 127.f / peak;
+            float far = 0.f;  // the largest distance of a quotient from its code
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                uint32_t q[E];
+#pragma unroll
+                for (int j = 0; j < E; j++) {
+                    const float p = value(i * E + j), c = fmaf(p, inv, kMagic);
+                    q[j] = __float_as_uint(c);
+                    if (!kShort) far = fmaxf(far, fabsf(fmaf(p, inv, kMagic - c)));
+                }
+                if (in(i) && BPQ4K_CHECK(e0 + 32u * E * i + E <= a.K && row < a.M, a.status)) store_codes<E>(codes + 32 * E * i, q);
+            }
+            exactly = far > kNear;
+        }
+        if (exactly) {
+            const double by = 127.0 / (double)peak;
+#pragma unroll 1  // (and read again: the values need no registers up to here)
+            for (int i = 0; i < NV; i++) {
+                if (!in(i)) continue;
+                const Pack<T, E> again = load_pack<T, E>(x + 32 * E * i);
+                uint32_t q[E];
+#pragma unroll
+                for (int j = 0; j < E; j++) {
+                    const double p = to_float(again.v[j]);
+                    q[j] = exact_code(p, (double)peak, (int)floor(p * by));
+                }
+                if (BPQ4K_CHECK(e0 + 32u * E * i + E <= a.K && row < a.M, a.status)) store_codes<E>(codes + 32 * E * i, q);
+            }
+        }
+        return;
+    }
+
     // one product, or a few that round to the same float, is the largest: whoever holds it knows a exactly
-    if (NORM && (mine == top || tiny)) {
+    if (mine == top || tiny) {
         double big = 0.0;
 #pragma unroll
         for (int g = 0; g < PT / G; g++) {
@@ -280,30 +321,17 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(const __grid_constant__ R
         }
         atomicMax(&s_exact, (unsigned long long)__double_as_longlong(big));
     }
-    // 127 does not divide the mantissa of a
-    if (!NORM && sizeof(T) == 2 && !tiny && ((top & 0x7FFFFFu) | 0x800000u) % 127u) {
-        const float up = __fdiv_ru(127.f, peak);
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            uint32_t q[E];
-#pragma unroll
-            for (int j = 0; j < E; j++) q[j] = __float_as_uint(fmaf(value(i * E + j), up, kMagic));
-            if (in(i) && BPQ4K_CHECK(e0 + 32u * E * i + E <= a.K && row < a.M, a.status)) store_codes<E>(codes + 32 * E * i, q);
-        }
-        return;
-    }
     const float inv = tiny ? 0.f : 127.f / peak;
     const uint64_t inv2 = pair(inv, inv), magic2 = pair(kMagic, kMagic), minus2 = pair(-1.f, -1.f);
     float far = tiny ? 1.f : 0.f;  // the largest distance of a quotient from its code
 #pragma unroll
     for (int g = 0; g < PT / G; g++) {
         float w[G];
-        if constexpr (NORM) weights(g, w);
+        weights(g, w);
         uint32_t q[G];
 #pragma unroll
         for (int j = 0; j < G; j += 2) {
-            uint64_t p = pair(value(g * G + j), value(g * G + j + 1));
-            if constexpr (NORM) p = mul2(p, pair(w[j], w[j + 1]));
+            const uint64_t p = mul2(pair(value(g * G + j), value(g * G + j + 1)), pair(w[j], w[j + 1]));
             const uint64_t c = fma2(p, inv2, magic2);
             const float2 f = halves(c), d = halves(fma2(p, inv2, fma2(c, minus2, magic2)));
             q[j] = __float_as_uint(f.x), q[j + 1] = __float_as_uint(f.y);
@@ -316,20 +344,20 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(const __grid_constant__ R
                 store_codes<E>(codes + 32 * E * i, reinterpret_cast<const uint32_t(&)[E]>(q[l * E]));
         }
     }
-    if constexpr (NORM) __syncthreads();
+    __syncthreads();
     if (far > kNear) {
-        const double exact = NORM ? __longlong_as_double((long long)s_exact) : (double)peak, by = tiny ? 127.0 / exact : 0.0;
+        const double exact = __longlong_as_double((long long)s_exact), by = tiny ? 127.0 / exact : 0.0;
 #pragma unroll
         for (int g = 0; g < PT / G; g++) {
             float w[G];
-            if constexpr (NORM) weights(g, w);
+            weights(g, w);
             uint32_t q[G];
 #pragma unroll
             for (int j = 0; j < G; j++) {
-                const float s = value(g * G + j), p = NORM ? s * w[j] : s, c = fmaf(p, inv, kMagic), d = fmaf(p, inv, -(c - kMagic));
+                const float s = value(g * G + j), p = s * w[j], c = fmaf(p, inv, kMagic), d = fmaf(p, inv, -(c - kMagic));
                 q[j] = __float_as_uint(c);
                 if (tiny || fabsf(d) > kNear) {
-                    const double pp = NORM ? (double)s * (double)w[j] : (double)s;
+                    const double pp = (double)s * (double)w[j];
                     q[j] = exact_code(pp, exact, tiny ? (int)floor(pp * by) : __float2int_rn(c - kMagic) - (d < 0.f ? 1 : 0));
                 }
             }
@@ -355,16 +383,16 @@ cudaError_t launch_pt(const RowsI8Args& a, cudaStream_t stream) {
     return cudaLaunchKernelEx(&cfg, rows_i8_kernel<T, E, PT, false, false>, a);
 }
 
-// Values of a thread (us on B200; R: with a residual).  8: the shortest way through a row, for rows that have an SM each (1 x 4096
-// float R 3.2, with 16 3.4) and short rows (2048 x 768 float R 5.8, 7.2; 2048 x 1025 bfloat16 R, single accesses, 8.1, 9.6).  32:
-// most loads in flight per SM, for long rows and many (2048 x 8192 float R 39.9, with 16 42.0, with 8 46.6; bfloat16 R 26.8, 29.0,
-// 37.7; 2048 x 14336 float R 65.6, 74.1), but not with single accesses, whose 32 of each operand spill (2048 x 5001 half R 37.9,
-// with 16 22.8).  16: between (200 x 8192 float R 7.2, with 8 8.0, with 32 8.7; 4096 x 2048 bfloat16 R 14.4, 15.3, 15.6).
+// Values of a thread (us on B200; R: with a residual, Q: no norm).  8: the shortest way through a row, for rows that have an SM each
+// (1 x 4096 float R 3.0, with 16 3.4; Q 1.8, 2.0) and short rows (2048 x 768 float R 5.8, 7.2; 2048 x 1025 bfloat16 R, single
+// accesses, 8.1, 9.6; 4096 x 1024 float Q 5.3, 6.1).  16 for the others: most loads in flight with the warps to hide them (2048 x 8192
+// float R 34.9, with 8 45.4, with 32 39.9; bfloat16 R 27.3, 37.7, 26.5; 700 x 8192 bfloat16 R 11.8, 13.9, 12.9; 2048 x 14336 float Q
+// 26.7, with 32 38.0; 2048 x 5001 half R, single accesses, 22.8, with 32 37.9).  32 where 1024 threads need them.
 template <typename T, int E>
 cudaError_t launch_vec(const RowsI8Args& a, int sm_count, cudaStream_t stream) {
     const uint32_t sms = (uint32_t)sm_count;
     if (a.K <= 8192u && (a.M <= sms || a.K <= (E == 1 ? 2048u : 1024u))) return launch_pt<T, E, 8>(a, stream);
-    if (a.K <= 16384u && (E == 1 || a.K <= 4096u || a.M <= 2u * sms)) return launch_pt<T, E, 16>(a, stream);
+    if (a.K <= 16384u) return launch_pt<T, E, 16>(a, stream);
     return launch_pt<T, E, 32>(a, stream);
 }
 
