@@ -16,7 +16,7 @@
 //
 // Memory bound (13 bytes a value with a float residual stream).  A row's values stay in registers between the two halves
 // (statistics, codes), one CTA to a row, several rows to an SM, so that one row's loads overlap another's arithmetic; that runs on
-// pairs (.f32x2).  2048 x 8192 float with a residual: 35 us, 0.95 of the copy rate.  With 16-bit streams instructions bound it, some 20 a
+// pairs (.f32x2).  2048 x 8192 float with a residual: 35 us, 0.95 of the copy rate.  With 16-bit streams instructions bound it, 24 a
 // value (bfloat16 27 us, 0.66).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
