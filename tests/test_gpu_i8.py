@@ -251,6 +251,16 @@ def test_matmul_matches_the_definition(ctx, M, N, K, kind, with_bias):
     assert ctx.device_status() == 0
 
 
+@pytest.mark.parametrize("shares", range(1, 10))
+@pytest.mark.parametrize("M", [9, 16, 30, 48, 50, 77, 112, 128])
+def test_matmul_of_shared_tiles(ctx, M, shares):
+    """Few tiles, whose K range CTAs share where each has four steps of 128 codes and more; the last step is a short one."""
+    for N, K in ((200, shares * 512 - 20), (129 * (9 - min(shares, 8)), shares * 512 + 77)):
+        host, (xr, wr, bias) = make_product(M, N, K, M * 11 + shares, True)
+        check_product(ctx.matmul_i8(xr, wr, bias=bias), *host, "f32")
+    assert ctx.device_status() == 0
+
+
 @pytest.mark.parametrize("M", [1, 3, 20, 150, 400])
 @pytest.mark.parametrize("K", [131071, 131056])
 def test_matmul_of_the_largest_sums(ctx, M, K):
