@@ -9,9 +9,9 @@
 //
 // The most likely tokens cost the pass next to nothing.  Values are compared as 64-bit keys (the value in the order of unsigned
 // words, below it the inverted index: the larger key is the larger value or, among equal ones, the lower index; no two are equal).
-// The pass leaves the largest value of every block (1024 values, 512 bytes of them in short rows); the k best tokens lie in the k blocks that are first by largest value
-// and, among equal ones, by position: whatever lies elsewhere has a value of each of these before it.  These blocks are read once
-// more (a thread's own values, 16 bytes here and there, would cost 64 bytes of DRAM for each 16: 512 x 128256, 32 tokens, 77 us
+// The pass leaves the largest value of every block (1024 values, 512 bytes of them in short rows); the k best tokens lie in the k blocks
+// that are first by largest value and, among equal ones, by position: whatever lies elsewhere has a value of each of these before it.
+// These blocks, or the lines of 512 bytes in them that matter, are read once more (a thread's own values, 16 bytes here and there, would cost 64 bytes of DRAM for each 16: 512 x 128256, 32 tokens, 77 us
 // against 54).
 //
 // Few rows: CTAs of a cluster share a row, so that no working memory is needed; the first of them gathers.
@@ -159,8 +159,9 @@ __device__ __forceinline__ uint32_t place_of(const unsigned long long* keys, uin
     return place;
 }
 
-// FINE: a block is one access of a warp, else a step or more.
-template <typename T, bool TOP, bool FINE, uint32_t kThreads>
+// FINE: a block is one access of a warp (a line), else a step or more.  LINES: a block is a step, and the lines' largest values are
+// kept beside the blocks', so that only lines are read again that have a value like the k-th block's.
+template <typename T, bool TOP, bool FINE, bool LINES, uint32_t kThreads>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(const __grid_constant__ LogprobsArgs a, const uint32_t group) {
     constexpr uint32_t kWarps = kThreads / 32u;
     // (half of either: float 48.3 and 60.5 us for 512 x 128256, bfloat16 36.9 and 43.2; twice, bfloat16: 37.8)
@@ -189,6 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
     while (!FINE && (lines >> shift) >= kThreads) shift++;  // a thread to a block; fine ones are few enough (launch_type)
     const uint32_t blocks = (lines + (1u << shift) - 1u) >> shift;
     __shared__ __align__(16) unsigned long long s_keys[TOP ? kThreads : 1];  // of the blocks: the largest value, the position
+    __shared__ float s_line[LINES ? kThreads * U : 1];
     if (TOP && tid >= blocks) s_keys[tid] = 0ull;
 
     // the given tokens' logits, the first of each thread: fetched now, needed at the end
@@ -228,19 +230,20 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
             uint4 p[U];
             float mx = -kInf;
             const bool whole = v0 + (step + 1u) * kStep <= v1;
-            if (!FINE && whole) {
+            if (!FINE && !LINES && whole) {
 #pragma unroll
                 for (uint32_t u = 0; u < U; u++) p[u] = __ldg(xv + i + 32u * u);
                 mx = warp_max_nan(largest<U>(p, T(0.f)));
             } else {
 #pragma unroll
                 for (uint32_t u = 0; u < U; u++)
-                    if (i + 32u * u < v1) p[u] = __ldg(xv + i + 32u * u);
+                    if (whole || i + 32u * u < v1) p[u] = __ldg(xv + i + 32u * u);
 #pragma unroll
                 for (uint32_t u = 0; u < U; u++) {
                     const uint4 one[1] = {p[u]};
-                    const float line = warp_max_nan(i + 32u * u < v1 ? largest<1>(one, T(0.f)) : -kInf);
+                    const float line = warp_max_nan(whole || i + 32u * u < v1 ? largest<1>(one, T(0.f)) : -kInf);
                     mx = max_nan(mx, line);
+                    if (LINES && lane == u && BPQ4K_CHECK(step < kThreads, a.status)) s_line[step * U + u] = line;
                     if (TOP && FINE && lane == 0 && step * U + u < lines && BPQ4K_CHECK(lines <= kThreads, a.status)) s_keys[step * U + u] = make_key(line, step * U + u);
                 }
             }
@@ -262,7 +265,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
     __shared__ Stats s_stats[kWarps];
     __shared__ __align__(16) unsigned long long s_found[TOP ? kThreads : 1];
     __shared__ unsigned long long s_list[32];  // the first blocks, then the largest keys, in descending order; 0 behind the last
-    __shared__ uint32_t s_count;
+    __shared__ uint32_t s_count, s_lines;
+    __shared__ uint32_t s_again[LINES ? 32u * U : 1];  // the lines to be read again
     __shared__ __align__(16) unsigned long long c_keys[TOP ? kMaxGroup * 32u : 1];
     __shared__ Stats c_stats[kMaxGroup];
 #pragma unroll
@@ -270,6 +274,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
     if (lane == 0) s_stats[warp] = st;
     if constexpr (TOP) {
         if (tid < 32u) s_list[tid] = 0ull;
+        if (tid == 0) s_lines = 0u;
         __syncthreads();
         // the k first blocks
         const unsigned long long own = s_keys[tid];
@@ -282,7 +287,16 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
         // what a key has to exceed: the k-th block has a value like its largest, at its end if nowhere else
         unsigned long long least = 0ull;
         if (bound) least = make_key(key_value(bound), head + min(v1, v0 + ((key_index(bound) + 1u) << shift) * 32u) * E - 1u) - 1ull;
-        const uint32_t first_lines = __popc(__ballot_sync(kFull, best != 0ull)) << shift;  // (lane i has the i-th block; none behind the k-th)
+        uint32_t first_lines = __popc(__ballot_sync(kFull, best != 0ull)) << shift;  // (lane i has the i-th block; none behind the k-th)
+        if constexpr (LINES) {
+            const float like = bound ? key_value(bound) : -kInf;
+            for (uint32_t l = tid; l < first_lines; l += kThreads) {
+                const uint32_t line = key_index(s_list[l >> kLog]) * U + l % U;
+                if (line < lines && !(s_line[line] < like)) s_again[atomicAdd(&s_lines, 1u)] = line;
+            }
+            __syncthreads();
+            first_lines = s_lines;
+        }
         // Keys above `least` are collected, a few more than k as a rule.  Should they not fit, the k-th of those that did is a better
         // bound, and the blocks are read again.
         for (;;) {
@@ -301,10 +315,14 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
                 uint32_t at[R];
 #pragma unroll
                 for (uint32_t u = 0; u < R; u++) {
-                    const uint32_t l = l0 + u * kWarps, b = key_index(__shfl_sync(kFull, best, min(l >> shift, 31u)));
-                    at[u] = v1;
-                    if (l < first_lines) at[u] = v0 + ((b << shift) + (l & ((1u << shift) - 1u))) * 32u + lane;
-                    if (BPQ4K_CHECK(l >= first_lines || b < blocks, a.status) && at[u] < v1) p[u] = __ldg(xv + at[u]);
+                    const uint32_t l = l0 + u * kWarps;
+                    uint32_t line;
+                    if constexpr (LINES)
+                        line = s_again[min(l, 32u * U - 1u)];
+                    else
+                        line = (key_index(__shfl_sync(kFull, best, min(l >> shift, 31u))) << shift) + (l & ((1u << shift) - 1u));
+                    at[u] = l < first_lines ? v0 + line * 32u + lane : v1;
+                    if (BPQ4K_CHECK(l >= first_lines || line >> shift < blocks, a.status) && at[u] < v1) p[u] = __ldg(xv + at[u]);
                 }
 #pragma unroll
                 for (uint32_t u = 0; u < R; u++)
@@ -370,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
     }
 }
 
-template <typename T, bool TOP, bool FINE, uint32_t kThreads>
+template <typename T, bool TOP, bool FINE, bool LINES, uint32_t kThreads>
 cudaError_t launch_rows(const LogprobsArgs& a, uint32_t group, cudaStream_t stream) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(a.M * group);
@@ -381,7 +399,7 @@ cudaError_t launch_rows(const LogprobsArgs& a, uint32_t group, cudaStream_t stre
     attr[0].val.clusterDim.x = group, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = group > 1u ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, TOP, FINE, kThreads>, a, group);
+    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, TOP, FINE, LINES, kThreads>, a, group);
 }
 
 template <typename T>
@@ -389,12 +407,18 @@ cudaError_t launch_type(const LogprobsArgs& a, int sm_count, cudaStream_t stream
     // CTAs that share a row: while they are fewer than the machine holds at once, and a thread has 16 values
     uint32_t group = 1;
     while (group < kMaxGroup && (uint64_t)a.M * group * 2u <= 4ull * sm_count && a.V >= group * 2u * 4096u) group *= 2u;
-    if (!a.nTop) return launch_rows<T, false, false, 256>(a, group, stream);
+    if (!a.nTop) return launch_rows<T, false, false, false, 256>(a, group, stream);
     // fine blocks where a CTA's part of a row has fewer of the others than tokens are asked for
-    if (a.V / group >= a.nTop * kBlockValues) return launch_rows<T, true, false, 256>(a, group, stream);
+    if (a.V / group >= a.nTop * kBlockValues) {
+        // Lines cost the pass 5 us of 46 (512 x 128256 float), and the second read, of few of them, no longer grows with k: 5 tokens 51.9 us,
+        // without 47.8; 16 tokens 52.4, 52.5; 32 tokens 54.0, 59.5; 512 x 32000 float, 20 tokens 19.4, 23.6; bfloat16, 5 tokens 14.0, 13.8;
+        // 64 x 128256, four CTAs a row, 5 tokens 13.7, 14.3.  So: where k blocks are an eighth of the row.
+        if ((uint64_t)a.nTop * 8u * kBlockValues >= a.V / group && a.V / group <= 255u * kBlockValues) return launch_rows<T, true, false, true, 256>(a, group, stream);
+        return launch_rows<T, true, false, false, 256>(a, group, stream);
+    }
     // (512 x 4000 float: 128 threads 7.7 us, 256 8.7; 8 x 128256, eight CTAs a row: 11.0 and 9.0)
-    if (a.V / group > 4096u) return launch_rows<T, true, true, 256>(a, group, stream);
-    return launch_rows<T, true, true, 128>(a, group, stream);
+    if (a.V / group > 4096u) return launch_rows<T, true, true, false, 256>(a, group, stream);
+    return launch_rows<T, true, true, false, 128>(a, group, stream);
 }
 
 }  // namespace

@@ -115,6 +115,18 @@ def test_orders_and_ties(ctx, kind, order, V):
 
 
 @pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("V", [8 * 255 * 1024 - 5, 8 * 255 * 1024, 8 * 255 * 1024 + 3, 8 * 256 * 1024 + 9])
+@pytest.mark.parametrize("equal", [False, True])
+def test_long_rows_and_many_alternatives(ctx, kind, V, equal):
+    """Eight CTAs share a row, around the most blocks of 1024 values that each has a thread for."""
+    import torch
+
+    x = torch.zeros(1, V, device="cuda") if equal else torch.randn(1, V, device="cuda")
+    x[0, V // 3] = 7.5
+    check(ctx, x.to(dtype_of(kind)), None, 32)
+
+
+@pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("fill", ["-inf", "lowest"])
 @pytest.mark.parametrize("V", [50, 4099, 32003])
 def test_masked_rows(ctx, kind, fill, V):
