@@ -333,6 +333,24 @@ def test_every_16_bit_quotient(ctx, name, bits):
     np.testing.assert_array_equal(got, want)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("K,pad,offset", [(700, 0, 0), (701, 3, 1), (9000, 0, 0), (20000, 0, 0), (20001, 2, 3)])
+def test_16_bit_rows_full_of_borders(ctx, kind, K, pad, offset):
+    """A largest value whose mantissa 127 divides (254, and 1143 = 9 * 127 in half), and odd multiples of a 254th of it."""
+    import torch
+
+    rows = []
+    for peak, step, most in [(254.0, 1.0, 253)] + ([(1143.0, 4.5, 227)] if kind == "f16" else []):
+        row = np.resize(step * np.arange(1, most + 1, 2), K)
+        row[1::2] *= -1
+        row[K // 2] = peak
+        rows += [row, row / 1024]
+    x = torch.from_numpy(np.stack(rows)).to(dtype_of(kind))
+    assert torch.equal(x.double(), torch.from_numpy(np.stack(rows)))
+    codes, scales, _ = rows_reference(x.float().numpy(), None, None, 0.0)
+    check_rows(ctx.quantize_i8(place(x, kind, pad, offset)[1]), codes, scales, K)
+
+
 def test_rows_of_several_dimensions(ctx):
     """[batch, tokens, K] and a single row [K] are rows like any others."""
     import torch
