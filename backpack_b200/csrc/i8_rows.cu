@@ -85,9 +85,14 @@ constexpr float kNear = 0.5f - 3e-5f;  // a quotient further from its code than 
 
 constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: added to a quotient, it leaves the rounded quotient in the low byte
 
-// The code of 127 p / peak, which lies in [k, k + 1): on which side of k + 1/2 it is.
+// The code of 127 p / peak, which lies in [k, k + 1): on which side of k + 1/2 it is.  Single values have 24 bits, and a double holds
+// both sides of the comparison.  Products of two (PRODUCTS) have 48, so the sides can have 56 and are rounded: they compare like the
+// exact ones unless they round to the same double, and then their rests, which a multiply-add gives exactly, decide.
+template <bool PRODUCTS>
 __device__ __forceinline__ uint32_t exact_code(double p, double peak, int k) {
-    const double l = 254.0 * p, r = (double)(2 * k + 1) * peak;
+    const double n = 2 * k + 1;
+    double l = 254.0 * p, r = n * peak;
+    if (PRODUCTS && l == r) l = fma(254.0, p, -l), r = fma(n, peak, -r);
     return (uint32_t)(l < r || (l == r && (k & 1) == 0) ? k : k + 1);
 }
 
@@ -307,7 +312,7 @@ __global__ void __launch_bounds__(1024, NORM || (PT == 32 && E == 4) ? 1 : 2) ro
 #pragma unroll
                 for (int j = 0; j < E; j++) {
                     const double p = to_float(again.v[j]);
-                    q[j] = exact_code(p, (double)peak, (int)floor(p * by));
+                    q[j] = exact_code<false>(p, (double)peak, (int)floor(p * by));
                 }
                 if (BPQ4K_CHECK(e0 + 32u * E * i + E <= a.K && row < a.M, a.status)) store_codes<E>(codes + 32 * E * i, q);
             }
@@ -365,7 +370,7 @@ __global__ void __launch_bounds__(1024, NORM || (PT == 32 && E == 4) ? 1 : 2) ro
                 q[j] = __float_as_uint(c);
                 if (tiny || fabsf(d) > kNear) {
                     const double pp = (double)s * (double)w[j];
-                    q[j] = exact_code(pp, exact, tiny ? (int)floor(pp * by) : __float2int_rn(c - kMagic) - (d < 0.f ? 1 : 0));
+                    q[j] = exact_code<true>(pp, exact, tiny ? (int)floor(pp * by) : __float2int_rn(c - kMagic) - (d < 0.f ? 1 : 0));
                 }
             }
 #pragma unroll
