@@ -38,6 +38,7 @@ struct bpq4k_context {
     int prefill_variant = 0;  // BPQ4K_OPT_PREFILL_VARIANT
     int prefill_arg() const { return prefill_mode | (prefill_variant << 4); }  // what the launcher takes
     int prefill_min_m = 25;  // four 8-row slabs of the streaming kernel cost as much as one tensor-core pass
+    uint32_t i8_wait_polls = 0;  // BPQ4K_OPT_I8_WAIT_POLLS
     int rows_min_m = 0;  // 0: automatic; smallest M of the several-rows kernel (takes_rows_kernel)
     // Its working memory.  The first streams that make such calls keep a block each (the stream's identity, which is never
     // used again, tells them apart, not its handle); other streams' calls take theirs from the pool in stream order, which
@@ -554,6 +555,10 @@ int bpq4k_set_option(bpq4k_handle_t h, int option, int value) {
             if (value < 0) return fail(h, BPQ4K_ERR_INVALID_ARG, "rows_min_m must be >= 0");
             h->rows_min_m = value;
             return BPQ4K_OK;
+        case BPQ4K_OPT_I8_WAIT_POLLS:
+            if (value < 0) return fail(h, BPQ4K_ERR_INVALID_ARG, "i8_wait_polls must be >= 0");
+            h->i8_wait_polls = (uint32_t)value;
+            return BPQ4K_OK;
         case BPQ4K_OPT_STREAM_WARPS:
             if (value < 0 || value > 16) return fail(h, BPQ4K_ERR_INVALID_ARG, "stream warps must be 0..16");
             h->tune.warps = (uint32_t)value;
@@ -641,6 +646,7 @@ int bpq4k_get_option(bpq4k_handle_t h, int option, int* value) {
         case BPQ4K_OPT_STREAM_STAMPS: *value = (int)h->tune.stamp_launches; return BPQ4K_OK;
         case BPQ4K_OPT_PREFILL_MIN_M: *value = h->prefill_min_m; return BPQ4K_OK;
         case BPQ4K_OPT_ROWS_MIN_M: *value = h->rows_min_m; return BPQ4K_OK;
+        case BPQ4K_OPT_I8_WAIT_POLLS: *value = (int)h->i8_wait_polls; return BPQ4K_OK;
         case BPQ4K_OPT_LAST_MATMUL_KERNEL: *value = h->last_kernel; return BPQ4K_OK;
         case BPQ4K_OPT_STREAM_WARPS: *value = (int)h->tune.warps; return BPQ4K_OK;
         case BPQ4K_OPT_STREAM_KSPLIT: *value = (int)h->tune.wk; return BPQ4K_OK;
@@ -1112,7 +1118,7 @@ int bpq4k_matmul_i8(bpq4k_handle_t h, int ftype, const int8_t* X, const float* x
     DeviceGuard g(h->device);
     MatmulI8Args a{};
     a.X = X, a.xs = x_scales, a.W = W, a.ws = w_scales, a.bias = bias, a.Y = Y;
-    a.M = M, a.N = N, a.K = K, a.ldx = ldx, a.ldw = ldw, a.ldy = ldy, a.status = h->dev_status;
+    a.M = M, a.N = N, a.K = K, a.ldx = ldx, a.ldw = ldw, a.ldy = ldy, a.wait_polls = h->i8_wait_polls, a.status = h->dev_status;
     int launches = 0;
     const cudaError_t e = launch_matmul_i8(a, ftype, h->sm_count, static_cast<cudaStream_t>(stream), &launches);
     h->launches += (uint64_t)launches;

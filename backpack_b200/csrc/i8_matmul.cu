@@ -18,8 +18,9 @@
 // A CTA takes more than half of an SM's shared memory, so two that allocate tensor memory never meet on one SM: with kernels on
 // several streams no allocation waits for a CTA that waits in a cluster for a third.
 //
-// Every wait is bounded: on a time-out the role raises the CTA's abort flag and the device status word, waits return at once
-// from then on, copies and mmas in flight are waited for (bounded too), and all threads meet at the end.
+// Every wait is bounded: on a time-out the role raises the abort flag of every CTA of its cluster and the device status word, and
+// waits that would block return at once from then on.  All threads of the cluster meet at the end, where the flag is final: if it
+// is raised, copies and mmas in flight are waited for (bounded too), whichever role gave up, before tensor memory is freed.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -138,8 +139,12 @@ cudaError_t launch_stream(const MatmulI8Args& m, uint32_t wk_log, cudaStream_t s
 
 // ---- tensor cores -------------------------------------------------------------------------------------------------------
 
-constexpr uint32_t kWaitLimit = 1u << 21;
+#ifdef BPQ4K_DEBUG_CHECKS
+constexpr uint32_t kWaitLimit = 1u << 28;             // polls of some 20 ns
+#else
+constexpr uint32_t kWaitLimit = 1u << 21;             // polls of up to 4 us
 constexpr uint32_t kSuspendNs = 1000;
+#endif
 constexpr uint32_t kStep = 128;                       // codes of a row per ring stage: the swizzle's row
 constexpr uint32_t kEpilogueWarps = 8, kThreads = (4 + kEpilogueWarps) * 32;
 constexpr uint32_t kMaxStages = 12;
@@ -157,6 +162,7 @@ struct TcArgs {
     uint32_t splits;                        // CTAs that share a tile's K range (one CTA form)
     uint32_t in_ring;                       // where they exchange their sums: 1 the ring (once it is free), 0 behind the barriers
     uint32_t stages, tmem_cols;
+    uint32_t wait_limit;                    // polls after which a wait gives up
     int* status;
 };
 
@@ -167,8 +173,19 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ uint32_t mbar_try_wait(uint32_t bar, uint32_t parity) {
+// One poll.  The product build is suspended meanwhile, for 4 us at most, whatever time is asked for; the debug build is not, so that a
+// short limit ends waits anywhere in the kernel.  (A branch between the two in the product build: 2048 x 28672 x 8192 305 -> 336 us.)
+__device__ __forceinline__ uint32_t mbar_poll(uint32_t bar, uint32_t parity) {
     uint32_t ok;
+#ifdef BPQ4K_DEBUG_CHECKS
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+#else
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
@@ -176,28 +193,37 @@ __device__ __forceinline__ uint32_t mbar_try_wait(uint32_t bar, uint32_t parity)
         : "=r"(ok)
         : "r"(bar), "r"(parity), "r"(kSuspendNs)
         : "memory");
+#endif
     return ok;
-}
-// Bounded wait; false once the CTA is aborting (then at once: the caller carries on so that barriers stay matched).
-__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status) {
-    if (mbar_try_wait(bar, parity)) return true;
-    for (uint32_t i = 0; i < kWaitLimit; i++) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 63u) == 0u && *abort_flag) return false;
-    }
-    *abort_flag = 1;
-    if (status) atomicExch(status, kDeviceTimeout);
-    return false;
-}
-// The same for what is still in flight at the end: also waits while the CTA aborts.
-__device__ __forceinline__ void wait_in_flight(uint32_t bar, uint32_t parity) {
-    for (uint32_t i = 0; i < kWaitLimit; i++)
-        if (mbar_try_wait(bar, parity)) return;
 }
 __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
     uint32_t r;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
+}
+// Raises the abort flag of every CTA of the cluster (of this one, where there is no cluster).
+__device__ __forceinline__ void raise_abort(volatile int* abort_flag) {
+    const uint32_t at = smem_u32(const_cast<const int*>(abort_flag));
+    uint32_t ctas;
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
+    for (uint32_t q = 0; q < ctas; q++) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_addr(at, q)), "r"(1) : "memory");
+}
+// Bounded wait; false if it ran out, or at once if it would block while the cluster aborts (the caller carries on without what it
+// waited for, so that barriers of the CTA stay matched).
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int* abort_flag, const TcArgs& a) {
+    if (mbar_poll(bar, parity)) return true;
+    for (uint32_t i = 1; i < a.wait_limit; i++) {
+        if (mbar_poll(bar, parity)) return true;
+        if ((i & 63u) == 1u && *abort_flag) return false;
+    }
+    raise_abort(abort_flag);
+    if (a.status) atomicExch(a.status, kDeviceTimeout);
+    return false;
+}
+// The same for what is in flight when the cluster aborts.
+__device__ __forceinline__ void wait_in_flight(uint32_t bar, uint32_t parity) {
+    for (uint32_t i = 0; i < kWaitLimit; i++)
+        if (mbar_poll(bar, parity)) return;
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
@@ -295,10 +321,11 @@ __global__ void __launch_bounds__(kThreads, 2) matmul_i8_kernel(const __grid_con
     auto empty = [&](uint32_t s) { return bar0 + (kMaxStages + s) * 8u; };
     auto acc_full = [&](uint32_t b) { return bar0 + (2u * kMaxStages + b) * 8u; };
     auto acc_empty = [&](uint32_t b) { return bar0 + (2u * kMaxStages + 2u + b) * 8u; };
-    const uint32_t parts_bar = bar0 + (2u * kMaxStages + 4u) * 8u, done_bar = parts_bar + 8u, ready_bar = parts_bar + 24u;
-    static_assert((2u * kMaxStages + 8u) * 8u <= kBarBytes, "barrier area");
+    const uint32_t parts_bar = bar0 + (2u * kMaxStages + 4u) * 8u, done_bar = parts_bar + 8u, ready_bar = parts_bar + 24u, issued_at = parts_bar + 32u;
+    static_assert((2u * kMaxStages + 9u) * 8u <= kBarBytes, "barrier area");
     volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + off_bar + (2u * kMaxStages + 6u) * 8u);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + off_bar + (2u * kMaxStages + 6u) * 8u + 4u);
+    const uint32_t* issued_steps = reinterpret_cast<const uint32_t*>(base_ptr + off_bar + (2u * kMaxStages + 8u) * 8u);  // by either half
 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     uint32_t rank = 0;
@@ -350,11 +377,11 @@ __global__ void __launch_bounds__(kThreads, 2) matmul_i8_kernel(const __grid_con
             for (uint32_t t = first_tile; t < a.tiles && ok; t += step_tile) {
                 const uint32_t rt = t / a.m_tiles, n0 = (rt * CG + half) * 128u, m0 = (t - rt * a.m_tiles) * a.tile + half * (a.tile / CG);
                 for (uint32_t c = c0; c < c1; c++) {
-                    ok = it == 0 || wait_bar(empty(s), (it - 1u) & 1u, abort_flag, a.status);
+                    ok = it == 0 || wait_bar(empty(s), (it - 1u) & 1u, abort_flag, a);
                     if (!ok) break;
                     const uint32_t dst = base + s * sbytes, bar = full0 + s * 8u;
                     if (!BPQ4K_CHECK(s < a.stages && c < a.chunks && rt * CG * 128u < a.N, a.status)) {
-                        *abort_flag = 1, ok = false;
+                        raise_abort(abort_flag), ok = false;
                         break;
                     }
                     if (leader) mbar_expect_tx(full(s), CG * sbytes);
@@ -364,8 +391,8 @@ __global__ void __launch_bounds__(kThreads, 2) matmul_i8_kernel(const __grid_con
                     if (++s == a.stages) s = 0, it++;
                 }
             }
-            if (!ok && leader)  // aborting: nothing may still be written to shared memory after the exit
-                for (uint32_t i = issued > a.stages ? issued - a.stages : 0u; i < issued; i++) wait_in_flight(full(i % a.stages), (i / a.stages) & 1u);
+            for (uint32_t q = 0; q < CG; q++)  // (both of a pair know how far both came)
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_addr(issued_at + half * 4u, CG == 2 ? q : rank)), "r"(issued) : "memory");
         }
     } else if (warp == 1) {
         if (lane == 0 && leader) {
@@ -375,10 +402,10 @@ __global__ void __launch_bounds__(kThreads, 2) matmul_i8_kernel(const __grid_con
             bool ok = true;
             for (uint32_t t = first_tile; t < a.tiles && ok; t += step_tile, i++) {
                 const uint32_t buf = i & 1u, d = tmem + buf * a.tile;
-                ok = i < 2u || wait_bar(acc_empty(buf), ((i >> 1) - 1u) & 1u, abort_flag, a.status);
+                ok = i < 2u || wait_bar(acc_empty(buf), ((i >> 1) - 1u) & 1u, abort_flag, a);
                 fence_after();
                 for (uint32_t c = c0; c < c1 && ok; c++) {
-                    ok = wait_bar(full(s), it & 1u, abort_flag, a.status);
+                    ok = wait_bar(full(s), it & 1u, abort_flag, a);
                     if (!ok) break;
                     fence_after();
                     const uint64_t da = desc_128(base + s * sbytes), db = desc_128(base + s * sbytes + 128u * kStep);
@@ -389,16 +416,13 @@ __global__ void __launch_bounds__(kThreads, 2) matmul_i8_kernel(const __grid_con
                 }
                 if (ok) umma_commit<CG>(acc_full(buf));
             }
-            if (!ok) {
-                umma_commit<CG>(done_bar);
-                wait_in_flight(done_bar, 0u);
-            }
         }
     } else if (warp >= 4) {
         // ---------------- epilogue ----------------
         const uint32_t e = threadIdx.x - 128u, quad = warp & 3u, side = (warp - 4u) >> 2, r = quad * 32u + lane;
         T* Y = static_cast<T*>(a.Y);
         uint32_t i = 0;
+        bool ok = true;
         for (uint32_t t = first_tile; t < a.tiles; t += step_tile, i++) {
             const uint32_t rt = t / a.m_tiles, n = (rt * CG + half) * 128u + r, m0 = (t - rt * a.m_tiles) * a.tile, buf = i & 1u;
             const uint32_t cols = min(a.tile, a.M - m0);
@@ -407,8 +431,8 @@ __global__ void __launch_bounds__(kThreads, 2) matmul_i8_kernel(const __grid_con
             float* xscale = scale + buf * kMaxTile;
             if (e < cols) xscale[e] = __ldg(a.xs + m0 + e);
             epilogue_sync();
-            // (a whole warp reads tensor memory, or none of it)
-            const bool ok = __all_sync(0xFFFFFFFFu, wait_bar(acc_full(buf), (i >> 1) & 1u, abort_flag, a.status));
+            // (a whole warp reads tensor memory, or none of it; after a wait that ran out it reads no more, stores no more and arrives nowhere)
+            ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(acc_full(buf), (i >> 1) & 1u, abort_flag, a));
             fence_after();
             const uint32_t acc = tmem + ((quad * 32u) << 16) + buf * a.tile;
             if (CG == 2 || a.splits == 1u) {
@@ -443,15 +467,15 @@ __global__ void __launch_bounds__(kThreads, 2) matmul_i8_kernel(const __grid_con
                 }
                 fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(peer_addr(acc_empty(buf), CG == 2 ? 0u : rank));
+                if (lane == 0 && ok) mbar_arrive_cluster(peer_addr(acc_empty(buf), CG == 2 ? 0u : rank));
             } else {
                 // every CTA of the cluster has a part of each sum: CTA q adds up and stores the columns that are q modulo the CTAs
                 const uint32_t mask = a.splits - 1u, log = 31u - __clz(a.splits), cols_each = a.tile >> log;
                 const uint32_t slot = base + off_exchange + (part * cols_each * 128u + r) * 4u;
                 bool ready = ok;
-                if (a.in_ring) {  // this CTA's mmas are done with its ring; the others'?
+                if (a.in_ring && ok) {  // this CTA's mmas are done with its ring; the others'?
                     if (e < a.splits) mbar_arrive_cluster(peer_addr(ready_bar, e));
-                    ready = __all_sync(0xFFFFFFFFu, wait_bar(ready_bar, 0u, abort_flag, a.status)) && ok;
+                    ready = __all_sync(0xFFFFFFFFu, wait_bar(ready_bar, 0u, abort_flag, a));
                 }
                 // (tiles of 16 columns: eight to either side)
                 auto send = [&](uint32_t c, const uint32_t* v, uint32_t n) {
@@ -473,8 +497,8 @@ __global__ void __launch_bounds__(kThreads, 2) matmul_i8_kernel(const __grid_con
                 }
                 asm volatile("fence.acq_rel.cluster;" ::: "memory");
                 __syncwarp();
-                if (lane < a.splits) mbar_arrive_cluster(peer_addr(parts_bar, lane));
-                const bool all = wait_bar(parts_bar, 0u, abort_flag, a.status);
+                if (lane < a.splits && ready) mbar_arrive_cluster(peer_addr(parts_bar, lane));
+                const bool all = ready && wait_bar(parts_bar, 0u, abort_flag, a);
                 const int* parts = reinterpret_cast<const int*>(base_ptr + off_exchange) + r;
                 if (all && live) {
 #pragma unroll 4
@@ -494,6 +518,27 @@ __global__ void __launch_bounds__(kThreads, 2) matmul_i8_kernel(const __grid_con
     fence_before();
     if (group > 1u) cluster_sync_all();  // nothing crosses over any more
     else __syncthreads();
+    if (*abort_flag) {  // (the same in the whole cluster)
+        if (warp == 0 && lane == 0) {
+            // A pair's copies are counted by the leader, whose barriers expect both halves of a step: whoever is behind issues as many
+            // steps as the other, whatever is in them.  The stages are free: the one ahead has seen the pair's mmas done with them.
+            const uint32_t steps = CG == 2 ? max(issued_steps[0], issued_steps[1]) : issued_steps[0];
+            for (uint32_t i = issued_steps[half]; i < steps; i++) {
+                const uint32_t s = i % a.stages, dst = base + s * sbytes, bar = (CG == 2 ? peer_addr(full(0), 0u) : full(0)) + s * 8u;
+                if (leader) mbar_expect_tx(full(s), CG * sbytes);
+                tma_load<CG>(dst, &a.tmap_w, 0u, 0u, bar);
+                tma_load<CG>(dst + 128u * kStep, &a.tmap_x, 0u, 0u, bar);
+            }
+            if (leader)
+                for (uint32_t i = steps > a.stages ? steps - a.stages : 0u; i < steps; i++) wait_in_flight(full(i % a.stages), (i / a.stages) & 1u);
+        } else if (warp == 1 && lane == 0) {
+            if (leader) umma_commit<CG>(done_bar);  // (of a pair: arrives in both)
+            wait_in_flight(done_bar, 0u);
+        }
+        __syncwarp();
+        if (group > 1u) cluster_sync_all();
+        else __syncthreads();
+    }
     if (warp == 2) {
         fence_after();
         if constexpr (CG == 1)
@@ -589,7 +634,7 @@ uint32_t max_clusters(uint32_t size, int sm_count) {
 template <int CG, typename T>
 cudaError_t launch_tc(const MatmulI8Args& m, const Cut& cut, int sm_count, cudaStream_t stream) {
     TcArgs a{};
-    a.xs = m.xs, a.ws = m.ws, a.bias = m.bias, a.Y = m.Y, a.M = m.M, a.N = m.N, a.ldy = m.ldy, a.status = m.status;
+    a.xs = m.xs, a.ws = m.ws, a.bias = m.bias, a.Y = m.Y, a.M = m.M, a.N = m.N, a.ldy = m.ldy, a.status = m.status, a.wait_limit = m.wait_polls ? m.wait_polls : kWaitLimit;
     a.chunks = (m.K + kStep - 1u) / kStep;
     if (cut.tiles > 0x7FFFFFFFull) return cudaErrorInvalidValue;
     a.tile = cut.tile, a.m_tiles = cut.m_tiles, a.tiles = (uint32_t)cut.tiles, a.splits = cut.splits;

@@ -190,6 +190,7 @@ struct MatmulI8Args {
     const float* bias;  // may be null
     void* Y;
     uint32_t M, N, K, ldx, ldw, ldy;
+    uint32_t wait_polls;  // 0, or after how many polls a wait inside the kernel gives up
     int* status;
 };
 cudaError_t launch_matmul_i8(const MatmulI8Args& a, int ftype, int sm_count, cudaStream_t stream, int* launches);

@@ -120,6 +120,10 @@ typedef enum bpq4k_option {
      * BPQ4K_OPT_PREFILL_MIN_M on it serves the F16X3 mode only, below it M <= 24.  Default 0: automatic, where it is the
      * faster kernel (never below 5 rows).  n > 0: every such M from n on; a large n: never. */
     BPQ4K_OPT_ROWS_MIN_M = 25,
+    /* How long a wait inside bpq4k_matmul_i8's kernels lasts before it gives up: the device status word then says
+     * BPQ4K_ERR_TIMEOUT, and the call's outputs are undefined.  0 (default): some seconds.  n > 0: n polls (of up to 4 us
+     * each; of some 20 ns in the debug build), so that a test can let waits run out.  No counterpart in the reference. */
+    BPQ4K_OPT_I8_WAIT_POLLS = 26,
     /* Read-only (bpq4k_get_option): how many times bpq4k_matmul_host_batch_f32 has recorded a dispatch
      * list into a replay graph on this handle.  A list is recorded again after any of the handle's
      * buffers had to grow. */
