@@ -403,10 +403,7 @@ cudaError_t launch_rows(const LogprobsArgs& a, uint32_t group, cudaStream_t stre
 }
 
 template <typename T>
-cudaError_t launch_type(const LogprobsArgs& a, int sm_count, cudaStream_t stream) {
-    // CTAs that share a row: while they are fewer than the machine holds at once, and a thread has 16 values
-    uint32_t group = 1;
-    while (group < kMaxGroup && (uint64_t)a.M * group * 2u <= 4ull * sm_count && a.V >= group * 2u * 4096u) group *= 2u;
+cudaError_t launch_group(const LogprobsArgs& a, uint32_t group, cudaStream_t stream) {
     if (!a.nTop) return launch_rows<T, false, false, false, 256>(a, group, stream);
     // fine blocks where a CTA's part of a row has fewer of the others than tokens are asked for
     if (a.V / group >= a.nTop * kBlockValues) {
@@ -419,6 +416,19 @@ cudaError_t launch_type(const LogprobsArgs& a, int sm_count, cudaStream_t stream
     // (512 x 4000 float: 128 threads 7.7 us, 256 8.7; 8 x 128256, eight CTAs a row: 11.0 and 9.0)
     if (a.V / group > 4096u) return launch_rows<T, true, true, false, 256>(a, group, stream);
     return launch_rows<T, true, true, false, 128>(a, group, stream);
+}
+
+template <typename T>
+cudaError_t launch_type(const LogprobsArgs& a, int sm_count, cudaStream_t stream) {
+    // CTAs that share a row: while they are fewer than the machine holds at once, and a thread has 16 values
+    uint32_t group = 1;
+    while (group < kMaxGroup && (uint64_t)a.M * group * 2u <= 4ull * sm_count && a.V >= group * 2u * 4096u) group *= 2u;
+    cudaError_t e = launch_group<T>(a, group, stream);
+    if (e != cudaSuccess && group > 1u) {  // a context that cannot place clusters (restricted SM sets): a CTA to a row
+        cudaGetLastError();
+        e = launch_group<T>(a, 1u, stream);
+    }
+    return e;
 }
 
 }  // namespace
