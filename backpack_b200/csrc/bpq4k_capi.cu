@@ -38,6 +38,7 @@ struct bpq4k_context {
     int prefill_variant = 0;  // BPQ4K_OPT_PREFILL_VARIANT
     int prefill_arg() const { return prefill_mode | (prefill_variant << 4); }  // what the launcher takes
     int prefill_min_m = 25;  // four 8-row slabs of the streaming kernel cost as much as one tensor-core pass
+    ClusterCounts i8_clusters;
     uint32_t i8_wait_polls = 0;  // BPQ4K_OPT_I8_WAIT_POLLS
     int rows_min_m = 0;  // 0: automatic; smallest M of the several-rows kernel (takes_rows_kernel)
     // Its working memory.  The first streams that make such calls keep a block each (the stream's identity, which is never
@@ -1118,7 +1119,7 @@ int bpq4k_matmul_i8(bpq4k_handle_t h, int ftype, const int8_t* X, const float* x
     DeviceGuard g(h->device);
     MatmulI8Args a{};
     a.X = X, a.xs = x_scales, a.W = W, a.ws = w_scales, a.bias = bias, a.Y = Y;
-    a.M = M, a.N = N, a.K = K, a.ldx = ldx, a.ldw = ldw, a.ldy = ldy, a.wait_polls = h->i8_wait_polls, a.status = h->dev_status;
+    a.M = M, a.N = N, a.K = K, a.ldx = ldx, a.ldw = ldw, a.ldy = ldy, a.clusters = &h->i8_clusters, a.wait_polls = h->i8_wait_polls, a.status = h->dev_status;
     int launches = 0;
     const cudaError_t e = launch_matmul_i8(a, ftype, h->sm_count, static_cast<cudaStream_t>(stream), &launches);
     h->launches += (uint64_t)launches;

@@ -25,8 +25,6 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include <atomic>
-
 #include "kernels.h"
 #include "q4k_common.cuh"
 
@@ -579,11 +577,13 @@ struct Cut {
 // An SM takes in about 92 GB/s (32 SMs streaming weights; 128 x 256 tiles of a pair), so a step costs what both operands' bytes of a
 // stage do; a shared tile costs an exchange.  (128 x 4096 x 14336: a pair 33 us, four CTAs to a tile 17.7.)
 constexpr uint32_t kSmem = 226u * 1024u;
-// Clusters of `size` CTAs (one an SM) that the device runs at once: not every SM of every GPC finds partners.
-uint32_t max_clusters(uint32_t size, int sm_count);
+
+// Clusters of `size` CTAs (one an SM) that the device runs at once: not every SM of every GPC finds partners.  0: none, or the
+// question failed (which is asked again then).  The answer is the handle's: it depends on the context that is current.
+uint32_t max_clusters(const MatmulI8Args& m, uint32_t size, int sm_count);
 
 template <int CG>
-Cut cut_of(const MatmulI8Args& m, int sm_count) {
+Cut cut_of(const MatmulI8Args& m, int sm_count, bool clusters) {
     Cut c{};
     const uint32_t most = CG == 1 ? kMaxTile / 2u : kMaxTile, unit = CG * 16u;  // (the mma's step of N)
     c.m_tiles = (m.M + most - 1u) / most;
@@ -592,9 +592,9 @@ Cut cut_of(const MatmulI8Args& m, int sm_count) {
     c.tiles = (uint64_t)((m.N + CG * 128u - 1u) / (CG * 128u)) * c.m_tiles;
     c.splits = 1;
     const uint32_t chunks = (m.K + kStep - 1u) / kStep;
-    if (CG == 1)
-        while (c.splits < kMaxSplits && c.tiles <= max_clusters(c.splits * 2u, sm_count) && chunks >= c.splits * 8u) c.splits *= 2u;
-    const uint64_t groups = CG * c.splits == 1u ? (uint32_t)sm_count : max_clusters(CG * c.splits, sm_count);
+    if (CG == 1 && clusters)
+        while (c.splits < kMaxSplits && c.tiles <= max_clusters(m, c.splits * 2u, sm_count) && chunks >= c.splits * 8u) c.splits *= 2u;
+    const uint64_t groups = CG * c.splits == 1u ? (uint32_t)sm_count : max_clusters(m, CG * c.splits, sm_count);
     if (groups == 0) {  // (a context whose SMs have no partners)
         c.us = 1e30;
         return c;
@@ -604,17 +604,13 @@ Cut cut_of(const MatmulI8Args& m, int sm_count) {
     return c;
 }
 
-uint32_t max_clusters(uint32_t size, int sm_count) {
-    static std::atomic<uint32_t> known[KernelConfig::kMaxDevices][4];  // (asked for once: a few calls a product, each some 0.1 us)
+uint32_t max_clusters(const MatmulI8Args& m, uint32_t size, int sm_count) {
+    uint32_t& known = m.clusters->known[size == 2u ? 0 : size == 4u ? 1 : 2];  // (asked for once: a few calls a product)
+    if (known) return known - 1u;
     static KernelConfig kcfg;
-    const uint32_t log = size == 2u ? 1u : size == 4u ? 2u : 3u, guess = (uint32_t)sm_count / size;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= KernelConfig::kMaxDevices) return guess;
-    if (const uint32_t n = known[dev][log].load(std::memory_order_relaxed)) return n - 1u;
     const void* func = reinterpret_cast<const void*>(matmul_i8_kernel<1, float>);
-    if (kcfg.prepare(func, kThreads, kSmem, nullptr) != cudaSuccess) return guess;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(guess * size);
+    cfg.gridDim = dim3((uint32_t)sm_count / size * size);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = kSmem;
     cudaLaunchAttribute attr[1];
@@ -623,11 +619,11 @@ uint32_t max_clusters(uint32_t size, int sm_count) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, func, &cfg) != cudaSuccess || n < 0) {
+    if (kcfg.prepare(func, kThreads, kSmem, nullptr) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, func, &cfg) != cudaSuccess || n < 0) {
         cudaGetLastError();
-        n = (int)guess;
+        return 0;
     }
-    known[dev][log].store((uint32_t)n + 1u, std::memory_order_relaxed);
+    known = (uint32_t)n + 1u;
     return (uint32_t)n;
 }
 
@@ -649,7 +645,7 @@ cudaError_t launch_tc(const MatmulI8Args& m, const Cut& cut, int sm_count, cudaS
     if (a.stages < 2u || smem_bytes(a.stages, a.tile, CG, exchange) <= 114u * 1024u || (a.in_ring && a.stages * stage_bytes(a.tile, CG) < exchange_bytes(a.tile))) return cudaErrorInvalidValue;
     a.tmem_cols = 32;
     while (a.tmem_cols < (a.splits > 1u ? 1u : 2u) * a.tile) a.tmem_cols *= 2u;
-    uint32_t groups = group == 1u ? (uint32_t)sm_count : max_clusters(group, sm_count);
+    uint32_t groups = group == 1u ? (uint32_t)sm_count : max_clusters(m, group, sm_count);
     if (a.splits > 1u || groups > a.tiles) groups = a.tiles;  // (a shared tile is a cluster's only one)
     if (!encode_rows(&a.tmap_w, m.W, m.N, m.K, m.ldw, 128u) || !encode_rows(&a.tmap_x, m.X, m.M, m.K, m.ldx, a.tile / CG)) return cudaErrorInvalidValue;
     const uint32_t smem = smem_bytes(a.stages, a.tile, CG, exchange);
@@ -679,9 +675,15 @@ cudaError_t launch_type(const MatmulI8Args& a, int sm_count, cudaStream_t stream
         while (wk_log < 4u && tiles << (wk_log + 1u) <= 32u * (uint64_t)sm_count && fetches >> (wk_log + 1u)) wk_log++;
         return wk_log == 4u ? launch_stream<T, 16>(a, wk_log, stream) : launch_stream<T, 8>(a, wk_log, stream);
     }
-    const Cut one = cut_of<1>(a, sm_count), pair = cut_of<2>(a, sm_count);
+    const Cut one = cut_of<1>(a, sm_count, true), pair = cut_of<2>(a, sm_count, true);
     // (of equals the one CTA form, which spreads over more SMs: 512 x 4096 x 4096 14.3 us, a pair 16.4)
-    return one.us <= pair.us ? launch_tc<1, T>(a, one, sm_count, stream) : launch_tc<2, T>(a, pair, sm_count, stream);
+    const bool single = one.us <= pair.us;
+    cudaError_t e = single ? launch_tc<1, T>(a, one, sm_count, stream) : launch_tc<2, T>(a, pair, sm_count, stream);
+    if (e != cudaSuccess && !(single && one.splits == 1u)) {  // another context than the one that was asked, which cannot place clusters
+        cudaGetLastError();
+        e = launch_tc<1, T>(a, cut_of<1>(a, sm_count, false), sm_count, stream);
+    }
+    return e;
 }
 
 }  // namespace

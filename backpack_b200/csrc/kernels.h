@@ -182,6 +182,9 @@ cudaError_t launch_rows_i8(const RowsI8Args& a, int ftype, int sm_count, cudaStr
 // X and W 16-byte aligned, ldx and ldw multiples of 16.
 constexpr uint32_t kMatmulI8MaxK = 131071;  // 128 * 128 * K stays below 2^31
 constexpr uint32_t kMatmulI8MaxRows = 1u << 24;
+struct ClusterCounts {
+    uint32_t known[3] = {};  // clusters of 2, 4 and 8 CTAs that the device runs at once, and one; 0: not asked yet
+};
 struct MatmulI8Args {
     const int8_t* X;
     const float* xs;
@@ -190,6 +193,7 @@ struct MatmulI8Args {
     const float* bias;  // may be null
     void* Y;
     uint32_t M, N, K, ldx, ldw, ldy;
+    ClusterCounts* clusters;  // the handle's
     uint32_t wait_polls;  // 0, or after how many polls a wait inside the kernel gives up
     int* status;
 };

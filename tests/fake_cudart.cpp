@@ -92,4 +92,13 @@ __attribute__((visibility("default"))) int fake_logprobs(int ftype, unsigned M, 
     a.M = M, a.V = a.ld = V, a.nTop = nTop;
     return (int)bpq4k::launch_logprobs(a, ftype, sm_count, nullptr);
 }
+// One handle's products: what it knows of clusters is kept between the calls, or forgotten (a new handle).
+__attribute__((visibility("default"))) int fake_matmul(int new_handle, int ftype, unsigned M, unsigned N, unsigned K, int sm_count) {
+    static bpq4k::ClusterCounts handle;
+    if (new_handle) handle = bpq4k::ClusterCounts();
+    bpq4k::MatmulI8Args a{};
+    a.M = M, a.N = N, a.K = K, a.ldx = a.ldw = (K + 15) / 16 * 16, a.ldy = N, a.clusters = &handle;
+    int launched = 0;
+    return (int)bpq4k::launch_matmul_i8(a, ftype, sm_count, nullptr, &launched);
+}
 }

@@ -48,3 +48,49 @@ def test_log_probabilities_without_clusters(fake, ftype, M, V, top, group):
     *refused, last = launches(fake)
     assert len(refused) == (group > 1) and all(r["refused"] for r in refused)
     assert not last["refused"] and last["cluster"] == 1 and last["grid"] == M and fake.fake_last_error() == 0
+
+
+# ---- the 8-bit matmul: (M, N, K), CTAs of a cluster on a whole device ---------------------------------------------------------
+
+PRODUCTS = [(13, 6144, 4096, 2), (64, 1024, 8192, 8), (100, 2048, 14336, 8), (2048, 28672, 8192, 2), (16, 128256, 4096, 1), (1, 1024, 4096, 1)]
+
+
+@pytest.mark.parametrize("ftype", [0, 1, 30])
+@pytest.mark.parametrize("M,N,K,cluster", PRODUCTS)
+def test_products_where_clusters_are_refused(fake, ftype, M, N, K, cluster):
+    fake.fake_reset(16, 0, 148)
+    assert fake.fake_matmul(1, ftype, M, N, K, 148) == 0
+    (one,) = launches(fake)
+    assert one["cluster"] == cluster
+    # a context that says so when it is asked: no launch with a cluster is tried
+    fake.fake_reset(1, 0, 148)
+    assert fake.fake_matmul(1, ftype, M, N, K, 148) == 0
+    (alone,) = launches(fake)
+    assert alone["cluster"] == 1 and not alone["refused"] and alone["grid"] >= 1
+    # a handle that has asked in a whole context, called in one that refuses
+    fake.fake_reset(16, 0, 148)
+    assert fake.fake_matmul(1, ftype, M, N, K, 148) == 0
+    fake.fake_reset(1, 0, 148)
+    assert fake.fake_matmul(0, ftype, M, N, K, 148) == 0
+    *refused, last = launches(fake)
+    assert len(refused) == (cluster > 1) and all(r["refused"] for r in refused)
+    assert last["cluster"] == 1 and not last["refused"] and last["name"] == alone["name"] and last["grid"] == alone["grid"] and fake.fake_last_error() == 0
+
+
+def test_what_a_restricted_context_answers_is_not_kept_for_others(fake):
+    fake.fake_reset(1, 0, 148)
+    assert fake.fake_matmul(1, 0, 2048, 28672, 8192, 148) == 0
+    fake.fake_reset(16, 0, 148)
+    assert fake.fake_matmul(1, 0, 2048, 28672, 8192, 148) == 0       # another handle
+    assert [l["cluster"] for l in launches(fake)] == [2]
+
+
+def test_a_failed_question_is_asked_again(fake):
+    fake.fake_reset(16, 2, 148)
+    assert fake.fake_matmul(1, 0, 2048, 28672, 8192, 148) == 0
+    assert [l["cluster"] for l in launches(fake)] == [1] and fake.fake_last_error() == 0
+    fake.fake_reset(16, 0, 148)
+    assert fake.fake_matmul(0, 0, 2048, 28672, 8192, 148) == 0
+    assert [l["cluster"] for l in launches(fake)] == [2]
+    asked = fake.fake_queries()
+    assert fake.fake_matmul(0, 0, 2048, 28672, 8192, 148) == 0 and fake.fake_queries() == asked      # and an answer is kept
