@@ -330,7 +330,10 @@ class Q4KContext:
         if t.device != self._dev:
             raise ValueError(f"{name} is not on {self._dev}")
         if t.dim() != 2:
-            t = t.view(-1, t.shape[-1])
+            try:
+                t = t.view(-1, t.shape[-1])
+            except (RuntimeError, IndexError):
+                raise ValueError(f"{name} of shape {tuple(t.shape)} and strides {t.stride()} is not rows at one distance from each other") from None
         ft = self._ftype.get(t.dtype)
         if t.dtype != dtype if dtype is not None else ft is None:
             raise ValueError(f"{name} is {t.dtype}, not {dtype or 'float32, float16 or bfloat16'}")
