@@ -11,10 +11,11 @@
 // words, below it the inverted index: the larger key is the larger value or, among equal ones, the lower index; no two are equal).
 // The pass leaves the largest value of every block (1024 values, 512 bytes of them in short rows); the k best tokens lie in the k blocks
 // that are first by largest value and, among equal ones, by position: whatever lies elsewhere has a value of each of these before it.
-// These blocks, or the lines of 512 bytes in them that matter, are read once more (a thread's own values, 16 bytes here and there, would cost 64 bytes of DRAM for each 16: 512 x 128256, 32 tokens, 77 us
-// against 54).
+// These blocks, or the lines of 512 bytes in them that matter, are read once more (a thread's own values, 16 bytes here and there,
+// would cost 64 bytes of DRAM for each 16: 512 x 128256, 32 tokens, 77 us against 54).
 //
-// Few rows: CTAs of a cluster share a row, so that no working memory is needed; the first of them gathers.
+// Few rows: CTAs of a cluster share a row, so that no working memory is needed; the first of them gathers.  Which values a thread
+// adds up, and so the last bits of S and T, follows from that and from where the row lies between 16-byte boundaries.
 //
 // What bounds it.  Float logits: DRAM (512 x 128256: 42 us without alternatives, 0.95 of the copy rate; 48 with five: a row's last
 // 5 us, the selection, have no other row to overlap).  16-bit logits: instructions, about 11 a value (32 us, 0.63; the exponentials

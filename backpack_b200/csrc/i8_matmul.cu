@@ -8,9 +8,10 @@
 //   one CTA    few activation rows.  Bound by reading the weights; CTAs of a cluster share the K range of a tile where there
 //              are fewer tiles than SMs, and each adds up and stores its share of the tile's columns.
 //   a pair     many activation rows (tcgen05 cta_group::2): each CTA loads half of either operand.
-// What bounds it (us; floor: the larger of the bytes at 6542 GB/s and the operations at twice the measured bfloat16 rate).
-// 2048 x 28672 x 8192: 285 to 300, floor 294: the tensor cores under the power cap.  1 x 128256 x 4096: 79, floor 80: DRAM.
-// Between, whole rounds of tiles (256 x 28672 x 8192: 112 tiles on 74 pairs, 58 against 41) and the 4.6 us from a kernel's start to
+// What bounds it (us; "against": the larger of the bytes at the measured copy rate, 6542 GB/s, and the operations at twice the
+// measured bfloat16 rate; a yardstick, not a bound: reads alone can run faster than a copy, and the clock varies under the power cap).
+// 2048 x 28672 x 8192: 292 to 305 against 294, the tensor cores under the power cap.  1 x 128256 x 4096: 79 against 80, DRAM.
+// Between, whole rounds of tiles (256 x 28672 x 8192: 112 tiles on 74 pairs, 57 against 41) and the 4.6 us from a kernel's start to
 // its first sum and from the last to the end (13 x 6144 x 4096: 9.2 against 3.9).
 // Roles (12 warps): warp 0 TMA, warp 1 mma, warp 2 tensor memory, warps 4-11 epilogue.  Persistent over the tiles; two
 // accumulators, so that a tile accumulates while the one before it is stored.

@@ -16,8 +16,9 @@
 //
 // Memory bound (13 bytes a value with a float residual stream).  A row's values stay in registers between the two halves
 // (statistics, codes), one CTA to a row, several rows to an SM, so that one row's loads overlap another's arithmetic; that runs on
-// pairs (.f32x2).  2048 x 8192 float with a residual: 35 us, 0.95 of the copy rate.  With 16-bit streams instructions bound it, 24 a
-// value (bfloat16 27 us, 0.66).
+// pairs (.f32x2).  2048 x 8192 float with a residual: 35 us, 0.95 of the copy rate.  With 16-bit streams (bfloat16 27 us, 0.67)
+// neither DRAM (55 % in the profile) nor the issue slots (50 %, 24 instructions a value) are full: warps wait for loads and at the
+// barrier between the halves, with too few rows on an SM to cover it.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -400,7 +400,8 @@ class Q4KContext:
         return out
 
     def i8_weight(self, w: Q4KWeight) -> I8Rows:
-        """A K-quant weight in 8 bits, a scale per output channel: dequantised some rows at a time and quantised again."""
+        """A K-quant weight in 8 bits, a scale per output channel: dequantised some rows at a time and quantised again.  K up to 32768
+        (quantize_i8's limit)."""
         torch = self._torch
         out = self._i8_out(w.N, w.K, None)[0]
         step = max(1, (16 << 20) // w.K)
@@ -432,7 +433,7 @@ class Q4KContext:
 
     def logprobs(self, logits, given=None, top: int = 0) -> LogProbs:
         """Log probabilities of given tokens ([M] or [M, G] int32), entropy and the `top` most likely tokens of each row of logits
-        [M, V] (bpq4k_logprobs)."""
+        [M, V] (bpq4k_logprobs).  Last bits depend on M and on the rows' alignment; top_ids do not."""
         torch = self._torch
         px, ft, m, v, ld = self._rows(logits, "logits")
         g, pg, plp, lp = 0, None, None, None

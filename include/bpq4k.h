@@ -446,8 +446,9 @@ int bpq4k_argmax_f32(bpq4k_handle_t h, const float* logits, uint32_t n, int32_t*
  * Element types of activations and logits are GGUF's numbers (runtime/gguf_loader.h:27-30).  Strides (ld...) are distances
  * between rows in elements, at least the row's length.  Rows of codes begin at multiples of 16 bytes and can be read to the next
  * multiple of 16 behind their K codes (the last row too); what lies there may be anything and is not written.
- * These calls allocate nothing, keep nothing and share nothing: they may be captured without a warm-up call, and calls on
- * different streams may overlap.  M = 0 does nothing.  Outputs may not overlap inputs except where it is said. */
+ * These calls allocate nothing and share nothing: they may be captured without a warm-up call, and calls on different streams may
+ * overlap.  A handle keeps how many clusters run at once in the context that is current when bpq4k_matmul_i8 first asks; where a
+ * context refuses clusters, calls do without them.  M = 0 does nothing.  Outputs may not overlap inputs except where it is said. */
 enum bpq4k_ftype { BPQ4K_TYPE_F32 = 0, BPQ4K_TYPE_F16 = 1, BPQ4K_TYPE_BF16 = 30 };
 
 /* Residual addition, root-mean-square norm, quantisation; for every row m:
@@ -457,14 +458,15 @@ enum bpq4k_ftype { BPQ4K_TYPE_F32 = 0, BPQ4K_TYPE_F16 = 1, BPQ4K_TYPE_BF16 = 30 
  *     codes = round(127 p / a)            to the nearest, ties to the even code: the exact quotient, whatever the order of sums
  *     scales = a / sqrt(mean(v^2) + eps) / 127
  * so that codes * scales is the norm's output.  A row of zeros has codes and scale 0.  A row in which a value or a product is
- * infinite or not a number has codes 0 and a NaN as its scale, which reaches everything that is made of it.  1 <= K <= 32768.
+ * infinite or not a number has codes 0 and a NaN as its scale, which reaches everything that is made of it.  1 <= K <= 32768
+ * (bpq4k_matmul_i8 takes longer rows, whose codes then come from elsewhere).
  * Replaces add_rms and the activation side of the Q8 dispatches (runtime/model_runner.cpp:3200-3243). */
 int bpq4k_add_rmsnorm_i8(bpq4k_handle_t h, int ftype, const void* X, const void* residual, const float* weight, float eps,
                          void* sum, int8_t* codes, float* scales, uint32_t M, uint32_t K, uint32_t ldx, uint32_t ldr,
                          uint32_t lds, uint32_t ldc, void* stream);
 
 /* The quantisation alone: codes = round(127 X / a), scales = a / 127, a = max |X| of the row.  For the inputs of projections
- * that follow no norm, and for weights at load time (a row per output channel). */
+ * that follow no norm, and for weights at load time (a row per output channel).  1 <= K <= 32768. */
 int bpq4k_quantize_i8(bpq4k_handle_t h, int ftype, const void* X, int8_t* codes, float* scales, uint32_t M, uint32_t K,
                       uint32_t ldx, uint32_t ldc, void* stream);
 
@@ -482,7 +484,9 @@ int bpq4k_matmul_i8(bpq4k_handle_t h, int ftype, const int8_t* X, const float* x
  *     top_ids[m][i], top_lp[m][i]                                 the nTop most likely tokens, descending, the lowest index first
  *                                                                 among equal ones; nTop <= 32 and <= V (0: not written)
  * Logits of -infinity are tokens of probability 0 (a mask); they come last among the alternatives.  A row that has nothing else: log
- * probabilities -infinity, entropy 0.  A row with a NaN or +infinity: NaNs, and -1 as ids. */
+ * probabilities -infinity, entropy 0.  A row with a NaN or +infinity: NaNs, and -1 as ids.
+ * Unlike bpq4k_matmul_i8's results, the last bits of given_lp, entropy and top_lp depend on the call: on M, and on where a row
+ * lies between 16-byte boundaries.  top_ids do not. */
 int bpq4k_logprobs(bpq4k_handle_t h, int ftype, const void* logits, uint32_t M, uint32_t V, uint32_t ld, const int32_t* given,
                    uint32_t nGiven, float* given_lp, float* entropy, uint32_t nTop, int32_t* top_ids, float* top_lp, void* stream);
 
